@@ -166,6 +166,52 @@ int kush_sm100_decode_fused_combine(int32_t head_dim, int32_t bits, int32_t page
                                     int32_t *counters, int32_t n_seqs, int32_t flags, const int32_t *order,
                                     void *stream);
 
+/* kush_sm100_decode_fused_combine under a sliding window with sink tokens: the query of sequence s, at position
+ * seq_lens[s] - 1, sees the last `window` tokens (itself among them) and the first `sinks` ones; window >= 1, sinks >= 0.
+ * Pages without a visible token are not read, nor their block-table entries (the caller may have given them back).
+ * counters: as there, or NULL to merge n_splits > 1 with kush_sm100_combine(_rotated).  Splits divide the visible pages.
+ * flags and order as kush_sm100_decode_ex (the rotated form takes the order here).  No counterpart in the reference. */
+int kush_sm100_decode_window(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group, const void *q,
+                             void *out, const void *cache, int64_t block_stride, int64_t head_stride,
+                             const void *tail_k, const int32_t *tail_idx, const int32_t *block_table,
+                             const int32_t *seq_lens, int64_t max_pages, int32_t hkv, float scale, int32_t n_splits,
+                             float *part_ml, float *part_o, int32_t *counters, int32_t n_seqs, int32_t flags,
+                             const int32_t *order, int32_t window, int32_t sinks, void *stream);
+
+/* Attention of several new rows per sequence (a prefill chunk, drafted tokens, one token) over the sequence's cached
+ * history and the new rows themselves, before kush_sm100_write stores them.  Replaces, as one call over the packed
+ * records, what kushkash does for T > 1 with torch (KushCache.attend_chunk and history_attention, kushkash/cache.py:
+ * 185-201 and _ops.py:309-339: page blocks dequantized, attended and merged).  Sequence s owns rows
+ * [query_start_loc[s], query_start_loc[s+1]) of q [rows][hkv*group][head_dim] (row stride q_stride), k_new and v_new
+ * [rows][hkv][head_dim] (row strides k_stride, v_stride) and out [rows][hkv*group][head_dim] (contiguous); seq_lens[s]
+ * counts them, the cache holds the ctx = seq_lens[s] - rows tokens before them.  Row t is at position ctx + t and sees
+ * the positions up to its own; with window > 0 of those only the last `window` (its own among them) and the first
+ * `sinks`.  History keys are c * ks + kb, the unfinished page's exact ones from tail_k[tail_idx[s]]; history values
+ * c * vs + vb; new rows enter as they are.  Pages that no row of the chunk sees are not read, nor their block-table
+ * entries.  Rows at and behind query_start_loc[n_seqs] are neither read nor written.
+ * n_splits > 1 divides each row tile's keys over that many blocks and merges them with a second kernel: part_ml
+ * [n_rows][hkv][n_splits][group][2], part_o [n_rows][hkv][n_splits][group][head_dim] fp32. */
+int kush_sm100_attend_chunk(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group, const void *q,
+                            int64_t q_stride, const void *k_new, const void *v_new, int64_t k_stride, int64_t v_stride,
+                            void *out, const int32_t *query_start_loc, const int32_t *seq_lens, const int32_t *tail_idx,
+                            const void *cache, int64_t block_stride, int64_t head_stride, const void *tail_k,
+                            const int32_t *block_table, int64_t max_pages, int32_t hkv, float scale, int32_t window,
+                            int32_t sinks, int32_t n_splits, float *part_ml, float *part_o, int64_t n_rows,
+                            int32_t n_seqs, void *stream);
+
+/* Rotary positions of `rows` rows of q (q_heads heads of head_dim) and k (k_heads; either count may be 0): channels
+ * [0, rotary_dim) of a head turn in pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved, by positions[row]
+ * (int32, or int64 if positions_64) times turns[i] / 2^64 of a full turn (device, rotary_dim / 2 entries; the product is
+ * taken modulo 2^64: exact for every position), times `factor`; the other channels are copied.  fp32 arithmetic, one
+ * rounding.  Strides in elements; an output may be its input (same strides).  No counterpart kernel in the reference
+ * (its callers rotate with torch before kush_append / kush_write). */
+int kush_sm100_rope(int32_t head_dim, int32_t dtype, int32_t rotary_dim, int32_t interleaved, const void *q,
+                    int64_t q_row_stride, int64_t q_head_stride, void *q_out, int64_t qo_row_stride,
+                    int64_t qo_head_stride, int32_t q_heads, const void *k, int64_t k_row_stride,
+                    int64_t k_head_stride, void *k_out, int64_t ko_row_stride, int64_t ko_head_stride, int32_t k_heads,
+                    const void *positions, int32_t positions_64, const uint64_t *turns, float factor, int64_t rows,
+                    void *stream);
+
 /* Which decode kernel a configuration takes: 1 = tensor-core kernel (mma), 0 = CUDA-core kernel,
  * KUSH_ERR_UNSUPPORTED if neither is built.  Mirrors GpuConfig.tensor_cores (kushkash/_build.py:120-122). */
 int kush_sm100_decode_tensor_cores(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group);

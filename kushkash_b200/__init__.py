@@ -8,7 +8,9 @@ Two ways in:
   * kushkash_b200.Ops calls the C ABI directly (page size 16 or 32, fused rotation, launch order, split partials).
 """
 from ._build import PAGE, BuildError, GpuConfig
-from ._ops import Ops, record_bytes, split_factor
+from ._ops import Ops, chunk_split_factor, record_bytes, split_factor
+from ._rotary import Rotary, rotary_frequencies
 
-__all__ = ["PAGE", "BuildError", "GpuConfig", "Ops", "record_bytes", "split_factor"]
+__all__ = ["PAGE", "BuildError", "GpuConfig", "Ops", "Rotary", "chunk_split_factor", "record_bytes",
+           "rotary_frequencies", "split_factor"]
 __version__ = "0.2.0"

@@ -28,11 +28,15 @@ import torch
 
 from . import _cuda
 from ._build import PAGE, GpuConfig
+from ._rotary import Rotary, make_rotary
 
 _DTYPE_NAMES = {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32"}
 MAX_SPLITS = 256
 MIN_SPLIT_PAGES = 16
 LONG_SPLIT_PAGES = 100
+CHUNK_TILE = 256
+MIN_CHUNK_SPLIT = 256
+_I32_MAX = 2 ** 31 - 1
 
 
 def record_bytes(head_dim: int, bits: int, page: int = PAGE) -> int:
@@ -59,6 +63,14 @@ def split_factor(num_seqs: int, num_kv_heads: int, max_full_pages: int, sms: int
     if units * ns > 2 * sms and max_full_pages // ns < LONG_SPLIT_PAGES:
         ns = max(-(-2 * sms // units), min(ns, -(-max_full_pages // LONG_SPLIT_PAGES)))
     return ns
+
+
+def chunk_split_factor(num_rows: int, num_seqs: int, num_kv_heads: int, group: int, max_len: int, sms: int) -> int:
+    """Split factor of attend_chunk(): its blocks are one per (tile of CHUNK_TILE query rows, kv head); when they fill less
+    than half the SMs the keys of each are divided so that the SMs are filled once, with at least MIN_CHUNK_SPLIT tokens
+    a split and at most MAX_SPLITS of them."""
+    units = max(1, max(num_seqs, -(-num_rows * group // CHUNK_TILE)) * num_kv_heads)
+    return max(1, min(MAX_SPLITS, sms // units, max_len // MIN_CHUNK_SPLIT))
 
 
 def _pool(cache: torch.Tensor) -> tuple[int, int, int]:
@@ -217,9 +229,52 @@ class Ops:
                   v_new.data_ptr(), k_new.stride(0), v_new.stride(0), new_dst.data_ptr(), n_new, kp.data_ptr(),
                   vp.data_ptr(), int(bool(rot)))
 
+    # ---------------------------------------------------------------- rotary positions
+    def rotary(self, rotary_dim: int | None = None, theta: float = 10000.0, *, interleaved: bool = False,
+               scaling: dict | None = None) -> Rotary:
+        """A plan for rope(): the first rotary_dim channels (default all) of a head turn, in pairs (i, i + r/2) or,
+        interleaved, (2i, 2i + 1), with base frequencies theta^(-2i/r) and the long-context scaling of
+        rotary_frequencies().  Made once (a small device tensor); good for every position."""
+        return make_rotary(self.device, self.D, rotary_dim, theta, interleaved, scaling)
+
+    def rope(self, q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary,
+             q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None
+             ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+        """Rotary positions of the rows of a step, before append() / write() / attend_chunk(): q [rows, Hq, D] and k
+        [rows, H, D] (either may be None; row and head strides free, e.g. parts of q|k|v rows), row i at positions[i]
+        (int32 or int64, contiguous), into q_out and k_out (new tensors, or q and k themselves, or others of their
+        shapes).  Returns (q_out, k_out).  Angles are exact to fp32 for every position; one rounding to the dtype."""
+        D, rows = self.D, positions.numel()
+        _need(positions.dtype in (torch.int64, torch.int32) and positions.is_contiguous(),
+              "rope: positions must be contiguous int32 or int64")
+        _need(rotary.head_dim == D and rotary.turns.device == self.device,
+              f"rope: the plan must be one of rotary() for head_dim {D} on {self.device}")
+        args = []
+        outs = []
+        for x, y in ((q, q_out), (k, k_out)):
+            if x is None:
+                _need(y is None, "rope: an output without its input")
+                args += (None, 0, 0, None, 0, 0, 0)
+                outs.append(None)
+                continue
+            if y is None:
+                y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            _need(x.dtype == self.dtype and y.dtype == self.dtype, f"rope: rows must be {self.dtype}")
+            _need(x.dim() == 3 and x.shape[0] == rows and x.shape[2] == D and x.shape == y.shape and x.stride(2) == 1
+                  and y.stride(2) == 1, f"rope: rows must be [{rows}, heads, {D}] with contiguous channels, "
+                  "outputs of their inputs' shapes")
+            args += (x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(), y.stride(0), y.stride(1), x.shape[1])
+            outs.append(y)
+        self._run("kush_sm100_rope", D, self.cfg.dtype_code, rotary.rotary_dim, int(rotary.interleaved), *args,
+                  positions.data_ptr(), int(positions.dtype == torch.int64), rotary.turns.data_ptr(), rotary.factor, rows)
+        return outs[0], outs[1]
+
     # ---------------------------------------------------------------- decode
-    def splits(self, num_seqs: int, num_kv_heads: int, max_full_pages: int) -> int:
-        """Split-KV factor for this device (split_factor)."""
+    def splits(self, num_seqs: int, num_kv_heads: int, max_full_pages: int, *, window: int | None = None,
+               sinks: int = 0) -> int:
+        """Split-KV factor for this device (split_factor); under a window, of the pages a query sees."""
+        if window is not None:
+            max_full_pages = min(max_full_pages, -(-window // self.P) + 1 + -(-sinks // self.P))
         return split_factor(num_seqs, num_kv_heads, max_full_pages, self.sms)
 
     def work_size(self, num_seqs: int, num_kv_heads: int, n_splits: int, fused: bool = False) -> int:
@@ -241,18 +296,24 @@ class Ops:
     def decode(self, q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
                seq_lens: torch.Tensor, tail_idx: torch.Tensor, tail_k: torch.Tensor, scale: float, n_splits: int = 1,
                work: torch.Tensor | None = None, *, rotate: bool = False, order: torch.Tensor | None = None,
-               fused: bool = False) -> None:
+               fused: bool = False, window: int | None = None, sinks: int = 0) -> None:
         """out[s] = softmax-scaled attention of q[s] over the seq_lens[s] cached tokens of sequence s.  n_splits > 1
         splits each sequence's pages over CTAs (split-KV) and merges them with a second launch; it needs `work`
         (work_size() fp32 elements).  fused: the merge runs inside the decode launch instead (the last CTA of each
         (sequence, kv head) merges; the same output bit for bit); `work` then needs work_size(..., fused=True)
         elements whose last S * Hkv start at 0.  rotate: the cache holds rotated K / V; q is rotated inside the
         kernel and the output rotated back before its store.  order: a contiguous int32 permutation of the
-        sequences, CTA x then decoding sequence order[x] (longest_first()); the outputs do not depend on it."""
+        sequences, CTA x then decoding sequence order[x] (longest_first()); the outputs do not depend on it.
+        window: the query sees the last `window` tokens (its own among them) and the first `sinks`; pages without a
+        visible token are not read, nor their block-table entries (give splits() the same window and sinks)."""
         S, H = q.shape[0], tail_k.shape[1]
         ml = o = 0
         if n_splits > 1:
             ml, o = self._parts(S, H, n_splits, work, fused)
+        if window is not None or sinks:
+            self._decode_window(q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, ml, o, rotate,
+                                order, fused, window, sinks)
+            return
         if fused and n_splits > 1:
             if order is not None:
                 _need(order.dtype == torch.int32 and order.numel() == S and order.is_contiguous(),
@@ -293,6 +354,80 @@ class Ops:
         _need(order.dtype == torch.int32 and order.numel() == S and order.is_contiguous(),
               "decode: order must be a contiguous int32 permutation of the sequences")
         self._run("kush_sm100_decode_ex", *head, 1 if rotate else 0, order.data_ptr())
+
+    def _decode_window(self, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale: float, n_splits: int,
+                       part_ml: int, part_o: int, rotate: bool, order: torch.Tensor | None, fused: bool,
+                       window: int | None, sinks: int) -> None:
+        S, H = q.shape[0], tail_k.shape[1]
+        _need(window is not None and window >= 1 and sinks >= 0,
+              f"decode: window must be >= 1 and sinks >= 0 (sinks need a window), got {window} and {sinks}")
+        _need(order is None or (order.dtype == torch.int32 and order.numel() == S and order.is_contiguous()),
+              "decode: order must be a contiguous int32 permutation of the sequences")
+        counters = part_ml + 4 * S * H * n_splits * self.G * (self.D + 2) if fused and n_splits > 1 else None
+        self._run("kush_sm100_decode_window", *self._fmt, self.G, q.data_ptr(), out.data_ptr(), *_pool(cache),
+                  tail_k.data_ptr(), tail_idx.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+                  block_table.stride(0), H, float(scale), n_splits, part_ml or None, part_o or None, counters, S,
+                  1 if rotate else 0, order.data_ptr() if order is not None else None, min(window, _I32_MAX),
+                  min(sinks, _I32_MAX))
+        if n_splits > 1 and counters is None:
+            entry = "kush_sm100_combine_rotated" if rotate else "kush_sm100_combine"
+            self._run(entry, self.D, self.cfg.dtype_code, self.G, out.data_ptr(), part_ml, part_o, n_splits, H, S)
+
+    # ---------------------------------------------------------------- chunk attention
+    def chunk_splits(self, num_rows: int, num_seqs: int, num_kv_heads: int, max_len: int, *, window: int | None = None,
+                     sinks: int = 0) -> int:
+        """Split factor of attend_chunk() for this device: row tiles and kv heads that leave SMs free split their keys
+        (chunk_split_factor).  num_rows: the step's new rows; max_len: the longest sequence, new rows counted."""
+        if window is not None:
+            max_len = min(max_len, window + sinks + -(-num_rows // max(1, num_seqs)))
+        return chunk_split_factor(num_rows, num_seqs, num_kv_heads, self.G, max_len, self.sms)
+
+    def chunk_work_size(self, num_rows: int, num_kv_heads: int, n_splits: int) -> int:
+        """fp32 elements of attend_chunk()'s work buffer for n_splits > 1: the unnormalised outputs of every row and
+        split, then their (M, L) pairs."""
+        return num_rows * num_kv_heads * n_splits * self.G * (self.D + 2)
+
+    def attend_chunk(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                     query_start_loc: torch.Tensor, seq_lens: torch.Tensor, tail_idx: torch.Tensor, cache: torch.Tensor,
+                     block_table: torch.Tensor, tail_k: torch.Tensor, scale: float, n_splits: int = 1,
+                     work: torch.Tensor | None = None, *, window: int | None = None, sinks: int = 0) -> None:
+        """Causal attention of a step's new rows over the cached history and themselves, read from the packed records
+        (no unpacked copy); call it before write() stores the rows.  Sequence s owns rows [qsl[s], qsl[s+1]) of q
+        [rows, H * G, D], k and v [rows, H, D] (row strides free, head stride D) and out [rows, H * G, D]
+        (contiguous); seq_lens[s] counts them, as in write().  Any mix of chunk lengths, one token and no history
+        included; rows at and behind qsl[S] are left alone.  window, sinks: as in decode(), for every row from its own
+        position.  n_splits > 1 (chunk_splits()) divides each tile's keys over more blocks and needs `work`
+        (chunk_work_size() fp32 elements).  Over a rotated cache, give it fwht() of q, k and v (write() wants the
+        latter two as well) and take fwht() of out."""
+        D, rows, S, H = self.D, q.shape[0], seq_lens.numel(), k.shape[1]
+        _need(q.dtype == self.dtype and k.dtype == self.dtype and v.dtype == self.dtype and out.dtype == self.dtype
+              and tail_k.dtype == self.dtype, f"attend_chunk: q, k, v, out and tail_k must be {self.dtype}")
+        _need(q.dim() == 3 and q.shape[1] == H * self.G and q.shape[2] == D and q.stride(1) == D and q.stride(2) == 1,
+              f"attend_chunk: q must be [rows, H * {self.G}, {D}] with head stride {D}")
+        _need(k.shape == (rows, H, D) == tuple(v.shape) and k.stride()[1:] == (D, 1) == v.stride()[1:],
+              f"attend_chunk: k and v must be [{rows}, H, {D}] with head stride {D}")
+        _need(out.shape == q.shape and out.is_contiguous(), "attend_chunk: out must be contiguous, of q's shape")
+        _need(tail_k.dim() == 4 and tuple(tail_k.shape[1:]) == (H, self.P, D) and tail_k.is_contiguous(),
+              f"attend_chunk: tail_k must be contiguous [slots, {H}, {self.P}, {D}]")
+        _need(query_start_loc.dtype == seq_lens.dtype == tail_idx.dtype == block_table.dtype == torch.int32
+              and query_start_loc.is_contiguous() and seq_lens.is_contiguous() and tail_idx.is_contiguous()
+              and query_start_loc.numel() == S + 1 and tail_idx.numel() >= S and block_table.shape[0] >= S
+              and block_table.stride(1) == 1, "attend_chunk: query_start_loc [S + 1], seq_lens and tail_idx [S] must be "
+              "contiguous int32, block_table [S, pages] int32 with contiguous rows")
+        _need((window is None or window >= 1) and sinks >= 0 and (window is not None or sinks == 0),
+              f"attend_chunk: window must be >= 1 and sinks >= 0 (sinks need a window), got {window} and {sinks}")
+        part_o = part_ml = None
+        if n_splits > 1:
+            need = self.chunk_work_size(rows, H, n_splits)
+            _need(work is not None and work.dtype == torch.float32 and work.is_contiguous() and work.numel() >= need,
+                  f"attend_chunk: n_splits={n_splits} needs a contiguous fp32 work buffer of >= {need} elements")
+            part_o = work.data_ptr()
+            part_ml = part_o + 4 * rows * H * n_splits * self.G * D
+        self._run("kush_sm100_attend_chunk", *self._fmt, self.G, q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(),
+                  k.stride(0), v.stride(0), out.data_ptr(), query_start_loc.data_ptr(), seq_lens.data_ptr(),
+                  tail_idx.data_ptr(), *_pool(cache), tail_k.data_ptr(), *_table(block_table), H, float(scale),
+                  min(window, _I32_MAX) if window is not None else 0, min(sinks, _I32_MAX), n_splits, part_ml, part_o, rows,
+                  S)
 
     def longest_first(self, seq_lens: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """A launch order for decode(order=): the sequences by full pages, most first (one small kernel; compute it

@@ -1,0 +1,88 @@
+"""Rotary position plans: the frequencies of Ops.rope(), as turns per position in 64-bit fixed point.
+
+A pair's angle is position * frequency.  The kernel takes it modulo one turn in integers: turns[i] = frequency / (2 pi) *
+2^64, and position * turns[i] modulo 2^64 is the fraction of a turn, for any position; so a plan has no table over
+positions and no longest position.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None) -> tuple[list[float], float]:
+    """(radians per position of pair i, factor of the cosines and sines).  Base frequencies theta^(-2i / rotary_dim);
+    `scaling` stretches them for contexts longer than the trained one, in the keys model configurations use:
+      rope_type "linear"   factor: every frequency divided by it
+                "ntk"      factor: theta becomes theta * factor^(r / (r - 2)): the fastest pair unchanged, the slowest / factor
+                "yarn"     factor, original_max_position_embeddings [, beta_fast 32, beta_slow 1, attention_factor
+                           0.1 ln(factor) + 1]: pairs that turn more than beta_fast times over the original context kept,
+                           those below beta_slow divided by factor, a ramp over the pair's index between
+                "llama3"   factor, low_freq_factor, high_freq_factor, original_max_position_embeddings: the same with a ramp
+                           over the number of turns
+                "default"  none"""
+    if theta <= 0:
+        raise ValueError(f"rotary: theta must be positive, got {theta}")
+    r = rotary_dim
+    freq = [theta ** (-2 * i / r) for i in range(r // 2)]
+    if not scaling:
+        return freq, 1.0
+    kind = scaling.get("rope_type", scaling.get("type"))
+    try:
+        if kind == "default":
+            return freq, 1.0
+        factor = float(scaling["factor"])
+        if factor <= 0:
+            raise ValueError(f"rotary: factor must be positive, got {factor}")
+        if kind == "linear":
+            return [f / factor for f in freq], 1.0
+        if kind == "ntk":
+            if r <= 2:
+                raise ValueError("rotary: ntk scaling needs rotary_dim > 2")
+            base = theta * factor ** (r / (r - 2))
+            return [base ** (-2 * i / r) for i in range(r // 2)], 1.0
+        if kind == "yarn":
+            if theta == 1:
+                raise ValueError("rotary: yarn scaling needs theta != 1")
+            context = float(scaling["original_max_position_embeddings"])
+            at = [r * math.log(context / (beta * 2 * math.pi)) / (2 * math.log(theta))
+                  for beta in (float(scaling.get("beta_fast") or 32), float(scaling.get("beta_slow") or 1))]
+            lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), r - 1)
+            keep = [1 - min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0) for i in range(r // 2)]
+            scale = scaling.get("attention_factor")
+            if scale is None:
+                scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+            return [f / factor * (1 - w) + f * w for f, w in zip(freq, keep)], float(scale)
+        if kind == "llama3":
+            context = float(scaling["original_max_position_embeddings"])
+            low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+            if high <= low:
+                raise ValueError("rotary: high_freq_factor must be above low_freq_factor")
+            keep = [min(max((context * f / (2 * math.pi) - low) / (high - low), 0.0), 1.0) for f in freq]
+            return [f / factor * (1 - w) + f * w for f, w in zip(freq, keep)], 1.0
+    except KeyError as e:
+        raise ValueError(f"rotary: {kind} scaling needs {e.args[0]}") from None
+    raise ValueError(f"rotary: unknown scaling {kind!r} (linear, ntk, yarn, llama3 or default)")
+
+
+@dataclass(frozen=True)
+class Rotary:
+    """A plan made by Ops.rotary(): pass it to Ops.rope() of the same head_dim on the same device."""
+    head_dim: int
+    rotary_dim: int
+    interleaved: bool
+    factor: float                # of the cosines and sines
+    turns: torch.Tensor          # [rotary_dim / 2] int64 (the bits of uint64): turns per position * 2^64
+
+
+def make_rotary(device: torch.device, head_dim: int, rotary_dim: int | None, theta: float, interleaved: bool,
+                scaling: dict | None) -> Rotary:
+    r = head_dim if rotary_dim is None else int(rotary_dim)
+    if r < 2 or r > head_dim or r % 2:
+        raise ValueError(f"rotary: rotary_dim must be even and in [2, {head_dim}], got {rotary_dim}")
+    freq, factor = rotary_frequencies(r, float(theta), scaling)
+    bits = [round(f / (2 * math.pi) * 2 ** 64) % 2 ** 64 for f in freq]
+    turns = torch.tensor([b - 2 ** 64 if b >= 2 ** 63 else b for b in bits], dtype=torch.int64, device=device)
+    return Rotary(head_dim, r, bool(interleaved), factor, turns)

@@ -2,6 +2,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include "kush_attend.cuh"
 #include "kush_common.cuh"
 
 namespace kush {
@@ -33,7 +34,7 @@ int launch_decode_mma(int D, int bits, int P, int dtype, int G, const void* q, v
                       int64_t block_stride, int64_t head_stride, const void* tail_k, const int32_t* tail_idx,
                       const int32_t* block_table, const int32_t* seq_lens, int64_t max_pages, int32_t hkv, float scale,
                       int32_t n_splits, float* part_ml, float* part_o, int32_t n_seqs, int rot, const int32_t* order,
-                      int32_t* counters, cudaStream_t stream);
+                      int32_t* counters, int32_t window, int32_t sinks, cudaStream_t stream);
 
 }  // namespace kush
 
@@ -68,7 +69,7 @@ static int decode_any(int32_t head_dim, int32_t bits, int32_t page, int32_t dtyp
                                  const void* tail_k, const int32_t* tail_idx, const int32_t* block_table,
                                  const int32_t* seq_lens, int64_t max_pages, int32_t hkv, float scale, int32_t n_splits,
                                  float* part_ml, float* part_o, int32_t n_seqs, int rot, const int32_t* order,
-                                 void* stream, int32_t* counters = nullptr) {
+                                 void* stream, int32_t* counters = nullptr, int32_t window = 0, int32_t sinks = 0) {
     if (n_seqs < 0 || hkv < 1 || group < 1 || n_splits < 1)
         return set_error(KUSH_ERR_ARG, "kush_sm100_decode: n_seqs %d hkv %d group %d n_splits %d", n_seqs, hkv, group,
                          n_splits);
@@ -87,9 +88,35 @@ static int decode_any(int32_t head_dim, int32_t bits, int32_t page, int32_t dtyp
     if (decode_mma_supported(head_dim, bits, page, dtype, group))
         return launch_decode_mma(head_dim, bits, page, dtype, group, q, out, cache, block_stride, head_stride, tail_k,
                                  tail_idx, block_table, seq_lens, max_pages, hkv, scale, n_splits, part_ml, part_o,
-                                 n_seqs, rot, order, n_splits > 1 ? counters : nullptr, st);
+                                 n_seqs, rot, order, n_splits > 1 ? counters : nullptr, window, sinks, st);
     g_err[0] = 0;
-    int rc = launch_decode_simt_any(head_dim, bits, page, dtype, group, q, out, cache, block_stride, head_stride, tail_k,
+    int rc;
+    if (window > 0) {
+        AttendArgs a{};
+        a.q = q;
+        a.out = out;
+        a.q_stride = int64_t(hkv) * group * head_dim;
+        a.cache = static_cast<const uint8_t*>(cache);
+        a.block_stride = block_stride;
+        a.head_stride = head_stride;
+        a.tail_k = tail_k;
+        a.tail_idx = tail_idx;
+        a.block_table = block_table;
+        a.seq_lens = seq_lens;
+        a.max_pages = max_pages;
+        a.H = hkv;
+        a.G = group;
+        a.S = n_seqs;
+        a.sm_log2 = scale * 1.4426950408889634f;
+        a.window = window;
+        a.sinks = sinks;
+        a.n_splits = n_splits;
+        a.part_ml = part_ml;
+        a.part_o = part_o;
+        a.rot = rot;
+        rc = launch_attend_simt(head_dim, bits, page, dtype, a, n_seqs, st);
+    } else
+        rc = launch_decode_simt_any(head_dim, bits, page, dtype, group, q, out, cache, block_stride, head_stride, tail_k,
                                     tail_idx, block_table, seq_lens, max_pages, hkv, scale, n_splits, part_ml, part_o,
                                     n_seqs, rot, order, st);
     if (rc == KUSH_ERR_UNSUPPORTED && g_err[0] == 0)
@@ -147,4 +174,19 @@ extern "C" int kush_sm100_decode_fused_combine(int32_t head_dim, int32_t bits, i
     return decode_any(head_dim, bits, page, dtype, group, q, out, cache, block_stride, head_stride, tail_k, tail_idx,
                       block_table, seq_lens, max_pages, hkv, scale, n_splits, part_ml, part_o, n_seqs,
                       (flags & KUSH_DECODE_ROTATE) ? 1 : 0, order, stream, counters);
+}
+
+extern "C" int kush_sm100_decode_window(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group,
+                                        const void* q, void* out, const void* cache, int64_t block_stride,
+                                        int64_t head_stride, const void* tail_k, const int32_t* tail_idx,
+                                        const int32_t* block_table, const int32_t* seq_lens, int64_t max_pages, int32_t hkv,
+                                        float scale, int32_t n_splits, float* part_ml, float* part_o, int32_t* counters,
+                                        int32_t n_seqs, int32_t flags, const int32_t* order, int32_t window, int32_t sinks,
+                                        void* stream) {
+    if (flags & ~KUSH_DECODE_ROTATE) return set_error(KUSH_ERR_ARG, "kush_sm100_decode_window: unknown flags %d", flags);
+    if (window < 1 || sinks < 0)
+        return set_error(KUSH_ERR_ARG, "kush_sm100_decode_window: window %d must be >= 1, sinks %d >= 0", window, sinks);
+    return decode_any(head_dim, bits, page, dtype, group, q, out, cache, block_stride, head_stride, tail_k, tail_idx,
+                      block_table, seq_lens, max_pages, hkv, scale, n_splits, part_ml, part_o, n_seqs,
+                      (flags & KUSH_DECODE_ROTATE) ? 1 : 0, order, stream, counters, window, sinks);
 }

@@ -172,6 +172,44 @@ __device__ __forceinline__ SplitRange split_range(const int32_t* seq_lens, int n
     return {int64_t(p0), int64_t(p1), active, active && p1 == full};
 }
 
+// ------------------------------------------------------------------ sliding window with sink tokens
+// What the query of a sequence's last token sees of its n tokens under a window of the last w tokens and the first k
+// (the sinks): tokens [0, ns) and [lo, n).  Its visible full pages, in order: pages [0, a) hold the sinks, pages
+// [b, full) the window; a page between them is never touched (its block-table entry may be stale).
+struct VisiblePages {
+    int32_t ns, lo;      // tokens [0, ns) and [lo, n) are visible
+    int32_t a, b;        // full pages [0, a) and [b, full)
+    int32_t count;       // a + (full - b)
+    __device__ __forceinline__ int64_t page(int64_t i) const { return i < a ? i : i - a + b; }
+};
+
+__device__ __forceinline__ VisiblePages visible_pages(int32_t n, int32_t window, int32_t sinks, int P) {
+    VisiblePages v;
+    v.lo = max(0, n - window);
+    v.ns = min(sinks, v.lo);
+    const int32_t full = n / P;
+    v.b = min(v.lo / P, full);
+    v.a = min((v.ns + P - 1) / P, v.b);
+    v.count = v.a + full - v.b;
+    return v;
+}
+
+// split_range over the visible full pages (indices into VisiblePages::page)
+__device__ __forceinline__ SplitRange split_range_window(const int32_t* seq_lens, int n_seqs, const VisiblePages& own, int z,
+                                                         int n_splits, int32_t window, int32_t sinks, int P) {
+    const uint32_t full = uint32_t(own.count);
+    if (n_splits == 1) return {0, int64_t(full), true, true};
+    uint32_t mx = 0;
+    for (int i = threadIdx.x % WARP; i < n_seqs; i += WARP)
+        mx = max(mx, uint32_t(visible_pages(seq_lens[i], window, sinks, P).count));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const uint32_t q = max(1u, (mx + uint32_t(n_splits) - 1) / uint32_t(n_splits));
+    const uint32_t p0 = min(full, uint32_t(z) * q), p1 = min(full, p0 + q);
+    const bool active = z == 0 || p0 < full;
+    return {int64_t(p0), int64_t(p1), active, active && p1 == full};
+}
+
 // ------------------------------------------------------------------ split-KV merge
 // The combine of one (sequence, kv head, q head) at output dim d (kushkash/kush/gpu.mojo:469-491): ml points at the
 // first split's (m, l) (natural-log max, sum; split z at ml[2 z G]), po at the first split's unnormalised output

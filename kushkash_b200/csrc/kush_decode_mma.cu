@@ -399,15 +399,19 @@ __device__ __noinline__ void combine_if_last(int32_t* counters, int64_t sh, int 
 }
 
 // grid (S, Hkv, n_splits), block 128.  ROT: q rotated in the prologue and the output rotated back before its store;
-// ORD: CTA x works on sequence order[x] (separate instantiations, so the plain kernels keep their code)
-template <int D, int BITS, int P, int NT, class IN, bool ROT, bool ORD>
+// ORD: CTA x works on sequence order[x] (separate instantiations, so the plain kernels keep their code).
+// WIN: a sliding window with sink tokens.  The page loop walks the sequence's visible pages (VisiblePages) and reads no
+// other page nor its block-table entry; a 16-token tile with no visible token is skipped, and in the at most three tiles
+// that a border cuts the masked tokens' scores become -inf.  Every tile that is processed holds a visible token, so the
+// running max is finite after its first tile.  kb_ref is the K bias of the first visible page, for all splits alike.
+template <int D, int BITS, int P, int NT, class IN, bool ROT, bool ORD, bool WIN>
 __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB)) decode_mma_kernel(
     const IN* __restrict__ q, IN* __restrict__ out, const uint8_t* __restrict__ cache, int64_t block_stride,
     int64_t head_stride, const IN* __restrict__ tail_k, const int32_t* __restrict__ tail_idx,
     const int32_t* __restrict__ block_table, const int32_t* __restrict__ seq_lens, int64_t max_pages, int H, int G,
     float sm_log2, int n_splits, float* __restrict__ part_ml, float* __restrict__ part_o,
     const __grid_constant__ CUtensorMap tmap, int use_tma, uint32_t swz_m, int32_t rows_per_head, int32_t box_rows,
-    const int32_t* __restrict__ order, int32_t* __restrict__ counters) {
+    const int32_t* __restrict__ order, int32_t* __restrict__ counters, int32_t window, int32_t sinks) {
     using F = Fmt<D, BITS, P>;
     using L = Lay<D, BITS>;
     using C = MmaCfg<D, BITS, P, NT>;
@@ -421,12 +425,15 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
     float* qsm = reinterpret_cast<float*>(ring + C::RING);              // [G][D] q * scale * log2e
     float* kbr = qsm + G * D;                                           // [D] kb_ref
     __half* kb16 = reinterpret_cast<__half*>(kbr + D);                  // [D] kb_ref as fp16 (read in K pair order)
-    const int s = ORD ? order[blockIdx.x] : blockIdx.x, h = blockIdx.y, z = blockIdx.z;     // launch order
+    const int s = ORD || (WIN && order) ? order[blockIdx.x] : blockIdx.x, h = blockIdx.y, z = blockIdx.z;  // launch order
     const int wid = threadIdx.x / WARP, lane = threadIdx.x % WARP, g = lane >> 2, tid = lane & 3;
     const int64_t n = seq_lens[s];
     const int tail_n = int(n % P);
     const int64_t full = n / P;
-    const SplitRange sr = split_range(seq_lens, int(gridDim.x), s, z, n_splits, P);
+    const VisiblePages vis = WIN ? visible_pages(int32_t(n), window, sinks, P) : VisiblePages{};
+    const SplitRange sr = WIN ? split_range_window(seq_lens, int(gridDim.x), vis, z, n_splits, window, sinks, P)
+                              : split_range(seq_lens, int(gridDim.x), s, z, n_splits, P);
+    auto page_at = [&](int64_t i) -> int64_t { return WIN ? vis.page(i) : i; };       // logical page of range index i
     if (!sr.active) {                                                   // no pages here: an empty partial
         for (int hd = threadIdx.x; hd < G; hd += NW * WARP) {
             const int64_t pb = ((int64_t(s) * H + h) * n_splits + z) * G + hd;
@@ -453,7 +460,7 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
     uint8_t* wcodes = ring + wid * NS * C::CSTRIDE;                     // this warp's code (int4: record) slots
     uint8_t* wscl = ring + NW * NS * C::CODES + wid * NS * C::SCALES;   // and its scale slots (int8)
     uint64_t* wbar = bars + wid * NS;
-    auto bt_at = [&](int i) -> int32_t { return i < npw ? bt[mine0 + int64_t(i) * NW] : 0; };
+    auto bt_at = [&](int i) -> int32_t { return i < npw ? bt[page_at(mine0 + int64_t(i) * NW)] : 0; };
     int32_t btw = bt_at(lane), btn = bt_at(32 + lane);                 // block ids of my pages, 32 at a time
     const uint32_t codes_u = smem_u32(wcodes), scl_u = smem_u32(wscl), bar_u = smem_u32(wbar);
     const int32_t hrow = h * rows_per_head;                             // the record's first row in the tensor map
@@ -497,7 +504,8 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
         for (int i = threadIdx.x; i < G * D; i += NW * WARP) qsm[i] = to_f32(q[qbase + i]) * sm_log2;
     }
     // kb_ref: K bias of the sequence's first page (only when one is full; a tail-only sequence uses 0)
-    const uint8_t* rec0 = full > 0 ? hcache + int64_t(bt[0]) * block_stride : nullptr;
+    const bool any_page = WIN ? vis.count > 0 : full > 0;
+    const uint8_t* rec0 = any_page ? hcache + int64_t(bt[page_at(0)]) * block_stride : nullptr;
     for (int i = threadIdx.x; i < D; i += NW * WARP) {
         const __half kb = rec0 ? reinterpret_cast<const __half*>(rec0 + F::OFF_KB)[i] : __float2half_rn(0.0f);
         kbr[i] = __half2float(kb);
@@ -552,8 +560,12 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
         const uint8_t* scl = C::SPLIT ? wscl + slot * C::SCALES : codes + C::CODES;   // ks, kb, vs, vb
         // one 16-token tile at a time (P = 32 pages have two): QK, online softmax, PV.  The softmax is tile-granular,
         // which keeps the register footprint of both page sizes the same.
+        const int64_t tok0 = WIN ? page_at(mine0 + int64_t(i) * NW) * P : 0;    // the page's first token
 #pragma unroll
         for (int mtt = 0; mtt < MTT; mtt++) {
+            if constexpr (WIN) {
+                if (tok0 + mtt * 16 >= vis.ns && tok0 + mtt * 16 + 16 <= vis.lo) continue;    // no visible token
+            }
             float sc[NT][4];
             {
                 // the page's K scale and bias pairs for this lane's dims (K' = c * ks + (kb - kb_ref)); reloaded per
@@ -587,6 +599,19 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
                     sc[nt][1] = a01.y;
                     sc[nt][2] = a23.x;
                     sc[nt][3] = a23.y;
+                }
+            }
+            if constexpr (WIN) {
+                const int64_t t0 = tok0 + mtt * 16;
+                if (t0 < vis.lo && t0 + 16 > vis.ns) {                     // a border cuts this tile
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const int64_t t = t0 + g + 8 * r;
+                        if (t >= vis.ns && t < vis.lo) {
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) sc[nt][2 * r] = sc[nt][2 * r + 1] = -INFINITY;
+                        }
+                    }
                 }
             }
             // online softmax with a lazily moved max; lane holds tokens mtt*16 + g (+8), heads nt*8 + 2tid + {0,1}
@@ -729,7 +754,9 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
             for (int d = lane; d < D; d += WARP) qkref = fmaf(qh[d], kbr[d], qkref);
             qkref = warp_sum(qkref);
             float x = -INFINITY;
-            if (has_tail && lane < tail_n) {
+            const int64_t tt = full * P + lane;                          // (the tail's last token is always visible)
+            const bool seen = has_tail && lane < tail_n && (!WIN || tt < vis.ns || tt >= vis.lo);
+            if (seen) {
                 constexpr int VE = 16 / sizeof(IN);                      // elements per 16-byte load
                 float acc = 0.0f;
                 for (int d0 = 0; d0 < D; d0 += VE) {
@@ -741,7 +768,7 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
                 x = acc - qkref;
             }
             const float mx = warp_max(x);
-            const float p = (has_tail && lane < tail_n) ? fast_exp2(x - mx) : 0.0f;
+            const float p = seen ? fast_exp2(x - mx) : 0.0f;
             const float lsum = warp_sum(p);
             if (lane == 0) {
                 c_m[NW * G + hd] = has_tail ? mx : -INFINITY;
@@ -865,13 +892,14 @@ bool make_page_map(const void* cache, int64_t block_stride, int64_t head_stride,
     return true;
 }
 
-template <int D, int BITS, int P, int NT, class IN, bool ROT, bool ORD>
+template <int D, int BITS, int P, int NT, class IN, bool ROT, bool ORD, bool WIN = false>
 int launch_mma_rot(int G, const void* q, void* out, const void* cache, int64_t block_stride, int64_t head_stride,
                    const void* tail_k, const int32_t* tail_idx, const int32_t* block_table, const int32_t* seq_lens,
                    int64_t max_pages, int32_t hkv, float scale, int32_t n_splits, float* part_ml, float* part_o,
-                   int32_t n_seqs, const int32_t* order, int32_t* counters, cudaStream_t stream) {
+                   int32_t n_seqs, const int32_t* order, int32_t* counters, cudaStream_t stream, int32_t window = 0,
+                   int32_t sinks = 0) {
     using C = MmaCfg<D, BITS, P, NT>;
-    auto kern = decode_mma_kernel<D, BITS, P, NT, IN, ROT, ORD>;
+    auto kern = decode_mma_kernel<D, BITS, P, NT, IN, ROT, ORD, WIN>;
     CUtensorMap map;
     memset(&map, 0, sizeof(map));
     uint32_t swz_m = 0;
@@ -891,7 +919,7 @@ int launch_mma_rot(int G, const void* q, void* out, const void* cache, int64_t b
     launch_pdl(kern, grid, dim3(MMA_NW * WARP), C::SMEM, stream, static_cast<const IN*>(q), static_cast<IN*>(out),
                static_cast<const uint8_t*>(cache), block_stride, head_stride, static_cast<const IN*>(tail_k), tail_idx,
                block_table, seq_lens, max_pages, hkv, G, scale * 1.4426950408889634f, n_splits, part_ml, part_o, map,
-               tma ? 1 : 0, swz_m, rows_per_head, box_rows, order, counters);
+               tma ? 1 : 0, swz_m, rows_per_head, box_rows, order, counters, window, sinks);
     return check_launch("kush_sm100_decode (tensor cores)");
 }
 
@@ -899,7 +927,15 @@ template <int D, int BITS, int P, int NT, class IN>
 int launch_mma(int G, const void* q, void* out, const void* cache, int64_t block_stride, int64_t head_stride,
                const void* tail_k, const int32_t* tail_idx, const int32_t* block_table, const int32_t* seq_lens,
                int64_t max_pages, int32_t hkv, float scale, int32_t n_splits, float* part_ml, float* part_o,
-               int32_t n_seqs, int rot, const int32_t* order, int32_t* counters, cudaStream_t stream) {
+               int32_t n_seqs, int rot, const int32_t* order, int32_t* counters, int32_t window, int32_t sinks,
+               cudaStream_t stream) {
+    if (window > 0)
+        return rot ? launch_mma_rot<D, BITS, P, NT, IN, true, false, true>(
+                         G, q, out, cache, block_stride, head_stride, tail_k, tail_idx, block_table, seq_lens, max_pages, hkv,
+                         scale, n_splits, part_ml, part_o, n_seqs, order, counters, stream, window, sinks)
+                   : launch_mma_rot<D, BITS, P, NT, IN, false, false, true>(
+                         G, q, out, cache, block_stride, head_stride, tail_k, tail_idx, block_table, seq_lens, max_pages, hkv,
+                         scale, n_splits, part_ml, part_o, n_seqs, order, counters, stream, window, sinks);
     if (rot)                                          // (the rotated decode runs in the natural order)
         return launch_mma_rot<D, BITS, P, NT, IN, true, false>(G, q, out, cache, block_stride, head_stride, tail_k,
                                                                tail_idx, block_table, seq_lens, max_pages, hkv, scale,
@@ -923,7 +959,7 @@ int launch_decode_mma(int D, int bits, int P, int dtype, int G, const void* q, v
                       int64_t block_stride, int64_t head_stride, const void* tail_k, const int32_t* tail_idx,
                       const int32_t* block_table, const int32_t* seq_lens, int64_t max_pages, int32_t hkv, float scale,
                       int32_t n_splits, float* part_ml, float* part_o, int32_t n_seqs, int rot, const int32_t* order,
-                      int32_t* counters, cudaStream_t stream) {
+                      int32_t* counters, int32_t window, int32_t sinks, cudaStream_t stream) {
     auto go = [&](auto Dc, auto Bc, auto Pc, auto in) -> int {
         using IN = decltype(in);
         if constexpr (std::is_same_v<IN, float>) {
@@ -931,16 +967,16 @@ int launch_decode_mma(int D, int bits, int P, int dtype, int G, const void* q, v
         } else if constexpr (Dc.value == 256) {
             return launch_mma<Dc.value, Bc.value, Pc.value, 1, IN>(G, q, out, cache, block_stride, head_stride, tail_k,
                                                                    tail_idx, block_table, seq_lens, max_pages, hkv,
-                                                                   scale, n_splits, part_ml, part_o, n_seqs, rot, order, counters, stream);
+                                                                   scale, n_splits, part_ml, part_o, n_seqs, rot, order, counters, window, sinks, stream);
         } else {
             if (G <= 8)
                 return launch_mma<Dc.value, Bc.value, Pc.value, 1, IN>(G, q, out, cache, block_stride, head_stride,
                                                                        tail_k, tail_idx, block_table, seq_lens,
                                                                        max_pages, hkv, scale, n_splits, part_ml,
-                                                                       part_o, n_seqs, rot, order, counters, stream);
+                                                                       part_o, n_seqs, rot, order, counters, window, sinks, stream);
             return launch_mma<Dc.value, Bc.value, Pc.value, 2, IN>(G, q, out, cache, block_stride, head_stride, tail_k,
                                                                    tail_idx, block_table, seq_lens, max_pages, hkv,
-                                                                   scale, n_splits, part_ml, part_o, n_seqs, rot, order, counters, stream);
+                                                                   scale, n_splits, part_ml, part_o, n_seqs, rot, order, counters, window, sinks, stream);
         }
     };
     return dispatch_fmt(D, bits, P, dtype, go);
