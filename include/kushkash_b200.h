@@ -219,7 +219,8 @@ int kush_sm100_decode_tensor_cores(int32_t head_dim, int32_t bits, int32_t page,
 /* Bounded-wait watchdog of the kernels that wait: bit 0 set if a decode launch gave up waiting for a page copy (its
  * outputs were written as NaN), bit 1 if a bulk write gave up waiting for its input rows (the records of that
  * warp's remaining items were not written), bit 2 if a peer-gather wait gave up on a peer (kush_sm100_gather_wait:
- * the gathered outputs are incomplete); 0 if none.  clear != 0 resets the flags.
+ * the gathered outputs are incomplete), bit 3 if a chunk attention gave up a wait inside a block (that block's outputs
+ * were written as NaN); 0 if none.  clear != 0 resets the flags.
  * Synchronous (reads device variables); -1 on a CUDA error.  No counterpart in the reference, whose kernels have
  * no bounded waits. */
 int kush_sm100_device_error(int32_t clear);

@@ -106,7 +106,8 @@ def check(rc: int, what: str) -> None:
 
 def device_error(clear: bool = True) -> int:
     """Bounded-wait flags since the last clear: bit 0 a decode launch gave up (its outputs are NaN), bit 1 a bulk
-    write gave up (some of its records were not written), bit 2 a peer-gather wait gave up on a peer; 0 if none."""
+    write gave up (some of its records were not written), bit 2 a peer-gather wait gave up on a peer, bit 3 a
+    chunk attention gave up a wait (outputs of that block are NaN); 0 if none."""
     rc = lib().kush_sm100_device_error(int(clear))
     if rc < 0:
         raise RuntimeError("kush_sm100_device_error: CUDA error")

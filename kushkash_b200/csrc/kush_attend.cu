@@ -128,7 +128,8 @@ extern "C" int kush_sm100_attend_chunk(int32_t head_dim, int32_t bits, int32_t p
     a.part_ml = part_ml;
     a.part_o = part_o;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int rc = launch_attend_simt(head_dim, bits, page, dtype, a, n_rows, st);
+    const int rc = attend_tc_supported(head_dim, dtype) ? launch_attend_tc(head_dim, bits, page, dtype, a, n_rows, st)
+                                                        : launch_attend_simt(head_dim, bits, page, dtype, a, n_rows, st);
     if (rc != KUSH_OK || n_splits == 1) return rc;
     return launch_chunk_combine(head_dim, dtype, a, n_rows, st);
 }

@@ -127,6 +127,9 @@ __device__ __forceinline__ int64_t part_row(const AttendArgs& a, int64_t row, in
     return ((row * a.H + h) * a.n_splits + z) * a.G + g;
 }
 
+// the tensor-core kernel (kush_attend_tc.cu): fp16 / bf16 rows, head_dim 64 or 128, any group
+int attend_tc_supported(int D, int dtype);
+int launch_attend_tc(int D, int bits, int P, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream);
 int launch_attend_simt(int D, int bits, int P, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream);
 
 }  // namespace kush

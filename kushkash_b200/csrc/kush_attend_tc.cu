@@ -1,0 +1,677 @@
+// Chunk attention on the 5th-generation tensor cores (fp16 / bf16 rows, head_dim 64 or 128).
+//
+// A block holds up to 256 query rows of one (sequence, kv head) and walks the 128-token key tiles they see.  Two slots
+// of 128 rows (M = 128 of tcgen05.mma) work in turn, so that one slot's products run under the other's softmax:
+//   paired  more than 128 rows: slot i holds rows [128 i, 128 i + 128); both read every key tile
+//   split   up to 128 rows (drafted tokens, short turns): both slots hold the same rows and take the key tiles in turn,
+//           each with its own running maximum, sum and output; merged at the end
+// Roles (16 warps of 128 registers, one block per SM): warps 0-3 and 4-7 the softmax of slots 0 and 1 (a thread per row),
+// warps 8-14 bring keys and values into shared memory (16-token units in turn: records dequantized, tail and new rows
+// converted; fp16), one thread of warp 15 issues the products:
+//   S[128 x 128] = Q K'^T   (both from shared memory, K-major, 128-byte swizzle), fp32 in TMEM
+//   O[128 x D]  += P V      (P fp16 in TMEM over the first half of S's columns, V from shared memory, N-major)
+// K' = c ks + (kb - ref), fp16, ref = the key bias of the first finished page the block sees: the same shift of every
+// score of a row, which the softmax drops; large channel offsets are gone before the rounding to fp16.  q and the new
+// rows enter as fp16 too (exact for bf16 within fp16's range, which the cache's own fp16 scales have as well).  Scores,
+// maxima, sums and outputs stay fp32; the weights p = 2^(s - m) <= 2^8 are rounded once to fp16.  The maximum moves
+// lazily: O is rescaled only when a score passes the maximum in use by 2^8.
+//
+// Waits are bounded (2 s): on a timeout the block raises the error flag, writes NaN and returns.
+#include "kush_async.cuh"
+#include "kush_attend.cuh"
+
+namespace kush {
+
+constexpr int TC_TM = 256, TC_TN = 128, TC_THREADS = 16 * WARP, TC_NPROD = 7;
+constexpr float TC_TAU = 8.0f;
+
+__device__ int g_attend_error = 0;
+
+template <int D>
+struct TcSmem {
+    static constexpr int BLK = 128 * 128;                    // 128 rows x 64 channels of fp16: one swizzled block
+    static constexpr int TILE = BLK * (D / 64);
+    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, REF = V + 2 * TILE;       // REF: fp32 [D]
+    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * 16, BYTES = MISC + 16 + 1024;   // + alignment
+};
+
+// ------------------------------------------------------------------ tcgen05 / TMEM helpers
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    // start address, leading and stride byte offsets (16-byte units), descriptor version 1, 128-byte swizzle
+    return uint64_t((addr & 0x3FFFF) >> 4) | uint64_t(lbo >> 4) << 16 | uint64_t(sbo >> 4) << 32 | uint64_t(1) << 46 |
+           uint64_t(2) << 61;
+}
+// kind::f16: fp32 accumulators, fp16 operands, A K-major, B K-major or (n_major) N-major
+__device__ __forceinline__ constexpr uint32_t instr_desc(int m, int n, bool n_major) {
+    return 1u << 4 | (n_major ? 1u << 16 : 0u) | uint32_t(n >> 3) << 17 | uint32_t(m >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc))
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc))
+                 : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// 32 columns of this warp's 32 lanes: thread = lane, register i = column i
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+            addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_pack(float lo, float hi) {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t h2_fma_u(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_sub_u(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t and_xor_u(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+
+// byte offset of (row, 8-channel chunk) in a tile of swizzled blocks
+__device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
+    return uint32_t((chunk >> 3) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ void st_chunk(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// The exact fp16 codes of 8 (int4: 16) channels.  int4: 8 bytes = channels 8 c .. + 7 in the low nibbles (lo), D/2 + 8 c ..
+// in the high ones (hi); int8: 16 bytes = channels 16 c .. + 7 (lo) and + 8 .. + 15 (hi).
+template <int BITS>
+__device__ __forceinline__ void codes_of(const uint32_t (&w)[BITS / 2], uint32_t (&lo)[4], uint32_t (&hi)[4]) {
+    if constexpr (BITS == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t x = prmt(w[i], 0, 0x3120);             // bytes b0 b2 b1 b3
+            const uint32_t y = x >> 8;                             // b2 b1 b3
+            lo[2 * i] = h2_sub_u(and_xor_u(x, 0x000F000Fu, 0x64086408u), 0x64086408u);
+            lo[2 * i + 1] = h2_sub_u(and_xor_u(y, 0x000F000Fu, 0x64086408u), 0x64086408u);
+            hi[2 * i] = h2_fma_u(and_xor_u(x, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u);
+            hi[2 * i + 1] = h2_fma_u(and_xor_u(y, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t u = w[i] ^ 0x80808080u;                 // signed code -> c + 128
+            uint32_t(&o)[4] = i < 2 ? lo : hi;
+            o[2 * (i & 1)] = h2_sub_u(prmt(u, 0x64646464u, 0x5140), 0x64806480u);
+            o[2 * (i & 1) + 1] = h2_sub_u(prmt(u, 0x64646464u, 0x7342), 0x64806480u);
+        }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void load_words(const uint8_t* p, T* w, int n) {          // n words (2 or 4), aligned to them
+    if (n == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+    }
+}
+
+// A 16-token unit of a key tile for one warp: lane = (row group rg, column c) holds rows RPL rg .. + RPL - 1, BPL bytes each.
+template <int D, int BITS, int P>
+struct Unit {
+    using F = Fmt<D, BITS, P>;
+    static constexpr int W = BITS / 2, BPL = 4 * W, LPR = F::DC / BPL, RG = WARP / LPR, RPL = 16 / RG;
+    // first chunks (8 channels) of the lane's lo and hi halves
+    __device__ static int lo_chunk(int c) { return BITS == 4 ? c : 2 * c; }
+    __device__ static int hi_chunk(int c) { return BITS == 4 ? c + D / 16 : 2 * c + 1; }
+};
+
+// grid (row tiles, Hkv, n_splits), block 512
+template <int D, int BITS, int P, class IN>
+__global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) {
+    using F = Fmt<D, BITS, P>;
+    using U = Unit<D, BITS, P>;
+    using M = TcSmem<D>;
+    constexpr int CH = D / 8;                                      // 8-channel chunks of a row
+    extern __shared__ uint8_t smem_raw[];
+    pdl_wait();
+    const int tid = threadIdx.x, wid = tid / WARP, lane = tid % WARP;
+    const int h = blockIdx.y, z = blockIdx.z;
+    RowTile t;
+    if (!row_tile(a, int(gridDim.x) - 1 - int(blockIdx.x), TC_TM, t)) return;      // later rows, more keys: first
+    const KeyTiles kt = key_tiles(t.p0, t.p1, a.window, a.sinks, TC_TN);
+    int i0, i1;
+    key_split(a, z, TC_TM, TC_TN, kt.count, i0, i1);
+    auto grow = [&](int r) { return t.q0 + (t.r0 + r) / a.G; };                    // global row of tile row r
+    auto ghead = [&](int r) { return (t.r0 + r) % a.G; };                          // its q head in the group
+    if (i0 >= i1) {                                                                // (n_splits > 1) empty partials
+        for (int r = tid; r < t.nr; r += TC_THREADS) {
+            float* ml = a.part_ml + 2 * part_row(a, grow(r), h, z, ghead(r));
+            ml[0] = -INFINITY;
+            ml[1] = 0.0f;
+        }
+        return;
+    }
+    const bool paired = t.nr > 128;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* sm = smem_raw + (base - smem_u32(smem_raw));
+    float* ref = reinterpret_cast<float*>(sm + M::REF);
+    const uint32_t bars = base + M::BARS;
+    const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64,
+                   p_full = bars + 80, o_full = bars + 96;                         // pairs: [stage] or [slot]
+    volatile int* gave_up = reinterpret_cast<volatile int*>(sm + M::MISC);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + M::MISC + 4);
+    if (tid == 0) {
+        uint64_t* b = reinterpret_cast<uint64_t*>(sm + M::BARS);
+        const int count[7] = {8, 1, 8, 1, 1, 4, 1};
+        for (int i = 0; i < 14; i++) mbar_init(b + i, count[i / 2]);
+        *gave_up = 0;
+        fence_mbar_init();
+    }
+    if (wid == 15) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // bounded wait; false if this block gave up
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        uint64_t t0 = 0;
+        for (uint32_t n = 0;; n++) {
+            uint32_t ok;
+            asm volatile(
+                "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                : "=r"(ok)
+                : "r"(bar), "r"(parity)
+                : "memory");
+            if (ok) return true;
+            if (*gave_up) return false;
+            if (n % 64 == 0) {
+                uint64_t now;
+                asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+                if (t0 == 0) t0 = now;
+                else if (now - t0 > 2000000000ull) {
+                    *gave_up = 1;
+                    atomicExch(&g_attend_error, 1);
+                    return false;
+                }
+            }
+        }
+    };
+    const int32_t* bt = a.block_table + int64_t(t.s) * a.max_pages;
+    const uint8_t* hcache = a.cache + int64_t(h) * a.head_stride;
+    const int full = t.ctx / P * P;                                                // cached tokens in finished pages
+    // the key reference: the bias of the first finished page that the row tile sees (the same for all its splits)
+    {
+        const int first = kt.a > 0 ? 0 : kt.lo / P * P;
+        const bool have = first < full;
+        const uint8_t* rec = have ? hcache + int64_t(bt[first / P]) * a.block_stride : nullptr;
+        if (tid < D) ref[tid] = have ? h_load(rec + F::OFF_KB, tid) : 0.0f;
+    }
+    // query rows to fp16, negated under a negative scale (the softmax multiplies by its magnitude)
+    {
+        const IN* q = static_cast<const IN*>(a.q);
+        const float sign = a.sm_log2 < 0.0f ? -1.0f : 1.0f;
+        for (int i = tid; i < t.nr * CH; i += TC_THREADS) {
+            const int r = i / CH, c = i % CH;
+            const uint4 raw = *reinterpret_cast<const uint4*>(q + grow(r) * a.q_stride + int64_t(h * a.G + ghead(r)) * D + 8 * c);
+            const IN* e = reinterpret_cast<const IN*>(&raw);
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = h2_pack(sign * to_f32(e[2 * j]), sign * to_f32(e[2 * j + 1]));
+            st_chunk(base + M::Q + (r >> 7) * M::TILE + tile_off(r & 127, c), w[0], w[1], w[2], w[3]);
+        }
+    }
+    fence_async();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_at;
+    // slot i's rows' positions, and whether it works on the key tile of index i
+    auto slot_p0 = [&](int i) { return paired && i == 1 ? t.ctx + (t.r0 + 128) / a.G : t.p0; };
+    auto slot_p1 = [&](int i) { return paired && i == 0 ? t.ctx + (t.r0 + 127) / a.G : t.p1; };
+    auto active = [&](int slot, int it) -> bool {
+        if (!paired) return ((it - i0) & 1) == slot;
+        const int j0 = kt.tile(it) * TC_TN;
+        if (j0 > slot_p1(slot)) return false;
+        const int lo = a.window > 0 ? max(0, slot_p0(slot) - a.window + 1) : 0;
+        return j0 + TC_TN > lo || j0 < a.sinks;
+    };
+    bool ok = true;
+
+    if (wid < 8) {
+        // ---------------------------------------------------------------- softmax: thread = row of its slot
+        const int slot = wid >> 2, row = (wid & 3) * WARP + lane, wrow = (wid & 3) * WARP;
+        const int r = paired ? slot * 128 + row : row;                             // tile row
+        const bool busy = (paired ? slot * 128 : 0) + wrow < t.nr;                 // this warp has rows
+        const int pos = t.ctx + (t.r0 + min(r, t.nr - 1)) / a.G;
+        const int wp0 = __shfl_sync(0xffffffffu, pos, 0), wp1 = __shfl_sync(0xffffffffu, pos, 31);
+        const float sc = fmaxf(fabsf(a.sm_log2), 1e-30f);                          // (a masked score stays -inf under scale 0)
+        const uint32_t lanes = uint32_t(wrow) << 16;
+        const uint32_t s_at = tmem + lanes + 128 * slot, o_at = tmem + lanes + 256 + 128 * slot;
+        float m = -INFINITY, l = 0.0f;
+        int n = 0;                                                                 // tiles done by this slot
+        for (int it = i0; it < i1; it++) {
+            if (!active(slot, it)) continue;
+            if (!wait(s_full + 8 * slot, n & 1)) {
+                ok = false;
+                break;
+            }
+            fence_after();
+            if (busy) {
+                const int j0 = kt.tile(it) * TC_TN;
+                // columns [0, hi] seen, and of those [lo, ...) or [0, sk)
+                const int hi = pos - j0, lo = a.window > 0 ? pos - a.window + 1 - j0 : -1, sk = a.sinks - j0;
+                const bool cut = j0 + TC_TN - 1 > wp0 || (a.window > 0 && j0 < wp1 - a.window + 1 && j0 + TC_TN > a.sinks);
+                auto load = [&](int c, uint32_t (&x)[32]) {
+                    tmem_ld32(s_at + 32 * c, x);
+                    wait_ld();
+                    if (cut) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const int col = 32 * c + i;
+                            if (col > hi || (col < lo && col >= sk)) x[i] = 0xFF800000u;      // -inf
+                        }
+                    }
+                };
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t x[32];
+                    load(c, x);
+                    float m4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) m4[i] = __uint_as_float(x[i]);
+#pragma unroll
+                    for (int i = 4; i < 32; i++) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(x[i]));
+                    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                }
+                mx *= sc;
+                const bool bump = mx > m + TC_TAU;                                 // (m = -inf: any score)
+                if (__any_sync(0xffffffffu, bump)) {
+                    const float mn = bump ? mx : m;
+                    const float corr = bump ? ex2(m - mn) : 1.0f;                  // first scores: 2^-inf = 0
+                    m = mn;
+                    l *= corr;
+                    if (n > 0) {                                                   // the slot's last product is done
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            uint32_t x[32];
+                            tmem_ld32(o_at + 32 * c, x);
+                            wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
+                            tmem_st32(o_at + 32 * c, x);
+                        }
+                    }
+                }
+                const float mm = m == -INFINITY ? 0.0f : m;                        // nothing seen yet: weights 0
+                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t x[32], p[16];
+                    load(c, x);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float e0 = ex2(fmaf(__uint_as_float(x[2 * i]), sc, -mm));
+                        const float e1 = ex2(fmaf(__uint_as_float(x[2 * i + 1]), sc, -mm));
+                        l4[i & 1] += e0;
+                        l4[2 + (i & 1)] += e1;
+                        p[i] = h2_pack(e0, e1);
+                    }
+                    tmem_st16(s_at + 16 * c, p);
+                }
+                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                wait_st();
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(p_full + 8 * slot);
+            n++;
+        }
+        // ---------------------------------------------------------------- the slot's output
+        if (ok && n > 0) {
+            ok = wait(o_full + 8 * slot, 0);
+            fence_after();
+        }
+        // split: slot 1 hands its maximum, sum and output over (in the key buffers, no longer read)
+        float* xm = reinterpret_cast<float*>(sm + M::K);                           // [2][128] m, l
+        float* xo = xm + 256;                                                      // [128][D + 4]
+        if (!paired) {
+            // both slots' products are done before the key buffers are reused
+            if (ok && slot == 1 && i1 - i0 > 0) ok = wait(o_full, 0);
+            if (slot == 1 && busy) {
+                xm[row] = n > 0 ? m : -INFINITY;
+                xm[128 + row] = l;
+                if (n > 0 && ok) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t x[32];
+                        tmem_ld32(o_at + 32 * c, x);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4*>(xo + row * (D + 4) + 32 * c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                    }
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        if (busy && (paired || slot == 0)) {
+            float mo = -INFINITY, f0 = 1.0f, f1 = 0.0f;
+            if (!paired) {
+                mo = xm[row];
+                const float mn = fmaxf(m, mo);
+                f0 = m == -INFINITY ? 0.0f : ex2(m - mn);
+                f1 = mo == -INFINITY ? 0.0f : ex2(mo - mn);
+                l = l * f0 + (f1 > 0.0f ? xm[128 + row] * f1 : 0.0f);
+                m = mn;
+            }
+            const bool real = r < t.nr;
+            const int64_t pr = real ? part_row(a, grow(r), h, z, ghead(r)) : 0;
+            const float inv = a.n_splits > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+            IN* o = real ? static_cast<IN*>(a.out) + ((grow(r) * a.H + h) * a.G + ghead(r)) * D : nullptr;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t x[32];
+                if (n > 0 && ok) {
+                    tmem_ld32(o_at + 32 * c, x);
+                    wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = ok ? 0u : 0x7FC00000u;
+                }
+                float y[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) y[i] = __uint_as_float(x[i]) * f0;
+                if (!paired && f1 > 0.0f) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) y[i] = fmaf(f1, xo[row * (D + 4) + 32 * c + i], y[i]);
+                }
+                if (!real) continue;
+                if (a.n_splits > 1) {
+                    float4* po = reinterpret_cast<float4*>(a.part_o + pr * D + 32 * c);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) po[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        alignas(16) IN e[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) e[j] = from_f32<IN>(y[i + j] * inv);
+                        *reinterpret_cast<uint4*>(o + 32 * c + i) = *reinterpret_cast<const uint4*>(e);
+                    }
+                }
+            }
+            if (real && a.n_splits > 1) {
+                a.part_ml[2 * pr] = ok ? m * 0.69314718055994531f : 0.0f;         // log2 units -> natural, for the combine
+                a.part_ml[2 * pr + 1] = l;
+            }
+        }
+        fence_before();
+    } else if (wid < 8 + TC_NPROD) {
+        // ---------------------------------------------------------------- keys and values into shared memory
+        const int c = lane % U::LPR, rg = lane / U::LPR;
+        const IN* tail = static_cast<const IN*>(a.tail_k) + (int64_t(a.tail_idx[t.s]) * a.H + h) * P * D;
+        const IN* kn = static_cast<const IN*>(a.k_new) + t.q0 * a.k_stride + int64_t(h) * D;
+        const IN* vn = static_cast<const IN*>(a.v_new) + t.q0 * a.v_stride + int64_t(h) * D;
+        const int lo_c = U::lo_chunk(c), hi_c = U::hi_chunk(c);
+        const bool flip = BITS == 8 ? (c >> 2) & 1 : D == 64 && (rg & 1);          // store order: spread the banks
+        uint32_t rf[8];                                                            // the reference of the lane's channels
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            rf[i] = h2_pack(ref[8 * lo_c + 2 * i], ref[8 * lo_c + 2 * i + 1]);
+            rf[4 + i] = h2_pack(ref[8 * hi_c + 2 * i], ref[8 * hi_c + 2 * i + 1]);
+        }
+        // the stream of units: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp takes every 7th
+        auto fill = [&](auto kvc, int n, int u) {
+            constexpr bool kv = decltype(kvc)::value;                              // values (else keys)
+            const int st = n & 1;
+            const int j0 = kt.tile(i0 + n) * TC_TN + 16 * u;                       // the unit's first token
+            const bool none = j0 > t.p1 || (j0 + 15 < kt.lo && j0 >= kt.ns);       // no row sees a token of it
+            const int kind = none ? 0 : j0 + 16 <= full ? 1 : j0 >= t.ctx && j0 + 15 <= t.p1 ? 2 : 3;
+            const uint32_t dst = base + (kv ? M::V : M::K) + st * M::TILE;
+            const uint32_t bar_e = (kv ? v_empty : k_empty) + 8 * st, bar_f = (kv ? v_full : k_full) + 8 * st;
+            if (kind == 1) {
+                const uint8_t* rec = hcache + int64_t(bt[j0 / P]) * a.block_stride;
+                const int row0 = j0 % P + U::RPL * rg;
+                uint32_t w[U::RPL][U::W];
+#pragma unroll
+                for (int i = 0; i < U::RPL; i++)
+                    load_words(rec + (kv ? F::OFF_VQ : 0) + (row0 + i) * F::DC + U::BPL * c, w[i], U::W);
+                uint32_t s[8], b[8];
+                if constexpr (!kv) {
+                    load_words(rec + F::OFF_KS + 16 * lo_c, s, 4);
+                    load_words(rec + F::OFF_KS + 16 * hi_c, s + 4, 4);
+                    load_words(rec + F::OFF_KB + 16 * lo_c, b, 4);
+                    load_words(rec + F::OFF_KB + 16 * hi_c, b + 4, 4);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) b[i] = h2_sub_u(b[i], rf[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < U::RPL; i++) {
+                        s[i] = uint32_t(reinterpret_cast<const uint16_t*>(rec + F::OFF_VS)[row0 + i]) * 0x10001u;
+                        b[i] = uint32_t(reinterpret_cast<const uint16_t*>(rec + F::OFF_VB)[row0 + i]) * 0x10001u;
+                    }
+                }
+                if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
+#pragma unroll
+                for (int i = 0; i < U::RPL; i++) {
+                    uint32_t lo[4], hi[4];
+                    codes_of<BITS>(w[i], lo, hi);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        lo[j] = h2_fma_u(lo[j], kv ? s[i] : s[j], kv ? b[i] : b[j]);
+                        hi[j] = h2_fma_u(hi[j], kv ? s[i] : s[4 + j], kv ? b[i] : b[4 + j]);
+                    }
+                    const int row = 16 * u + U::RPL * rg + i;
+                    if (flip) {
+                        st_chunk(dst + tile_off(row, hi_c), hi[0], hi[1], hi[2], hi[3]);
+                        st_chunk(dst + tile_off(row, lo_c), lo[0], lo[1], lo[2], lo[3]);
+                    } else {
+                        st_chunk(dst + tile_off(row, lo_c), lo[0], lo[1], lo[2], lo[3]);
+                        st_chunk(dst + tile_off(row, hi_c), hi[0], hi[1], hi[2], hi[3]);
+                    }
+                }
+            } else {
+                // new rows, the unfinished page, unseen tokens: 8-channel chunks of a row, CH lanes per row
+                constexpr int RPI = WARP / CH, NI = 16 / RPI;                      // rows per step, steps
+                const int cc = lane % CH;
+                uint4 raw[NI];
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const int j = j0 + i * RPI + lane / CH;
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (kind == 2 || (kind == 3 && kt.seen(j, t.p1) && j >= t.ctx)) {
+                        const IN* src = kv ? vn + int64_t(j - t.ctx) * a.v_stride : kn + int64_t(j - t.ctx) * a.k_stride;
+                        raw[i] = *reinterpret_cast<const uint4*>(src + 8 * cc);
+                    } else if (!kv && kind == 3 && kt.seen(j, t.p1) && j >= full) {
+                        raw[i] = *reinterpret_cast<const uint4*>(tail + (j % P) * D + 8 * cc);
+                    }
+                }
+                if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const int row = 16 * u + i * RPI + lane / CH, j = j0 + i * RPI + lane / CH;
+                    const IN* e = reinterpret_cast<const IN*>(&raw[i]);
+                    float x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x[k] = to_f32(e[k]);
+                    const bool see = kind == 2 || (kind == 3 && kt.seen(j, t.p1));
+                    if (kind == 3 && see && j < t.ctx && (kv || j < full)) {       // from a record, one by one
+                        const uint8_t* rec = hcache + int64_t(bt[j / P]) * a.block_stride;
+                        const int s = j % P;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const int d = 8 * cc + k;
+                            x[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + s * F::DC, d)), h_load(rec + F::OFF_VS, s),
+                                             h_load(rec + F::OFF_VB, s))
+                                      : fmaf(float(code_at<D, BITS>(rec + s * F::DC, d)), h_load(rec + F::OFF_KS, d),
+                                             h_load(rec + F::OFF_KB, d));
+                        }
+                    }
+                    if (!kv && see) {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) x[k] -= ref[8 * cc + k];
+                    }
+                    st_chunk(dst + tile_off(row, cc), h2_pack(x[0], x[1]), h2_pack(x[2], x[3]), h2_pack(x[4], x[5]),
+                             h2_pack(x[6], x[7]));
+                }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar_f);
+        };
+        for (int x = wid - 8; x < 16 * (i1 - i0) && ok; x += TC_NPROD) {
+            if (x & 8) fill(IC<1>{}, x >> 4, x & 7);
+            else fill(IC<0>{}, x >> 4, x & 7);
+            ok = __all_sync(0xffffffffu, ok);
+        }
+    } else if (lane == 0) {
+        // ---------------------------------------------------------------- the products, in the order of (tile, slot)
+        constexpr uint32_t ID_S = instr_desc(128, TC_TN, false), ID_O = instr_desc(128, D, true);
+        auto next = [&](int& it, int& slot) {                                      // the next active (tile, slot) pair
+            do {
+                if (++slot == 2) {
+                    slot = 0;
+                    it++;
+                }
+            } while (it < i1 && !active(slot, it));
+        };
+        auto last_user = [&](int slot, int it) { return slot == 1 || !active(1, it); };
+        int sit = i0, ss = -1, pit = i0, ps = -1;                                  // cursors of S and of O products
+        next(sit, ss);
+        next(pit, ps);
+        uint32_t done[2] = {0, 0};                                                 // O products issued per slot
+        auto issue_s = [&]() -> bool {
+            const int n = sit - i0, st = n & 1;
+            if (!wait(k_full + 8 * st, (n >> 1) & 1)) return false;
+            fence_after();
+            const uint32_t qa = base + M::Q + (paired && ss == 1 ? M::TILE : 0), ka = base + M::K + st * M::TILE;
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+                const uint32_t off = (k >> 2) * M::BLK + (k & 3) * 32;
+                mma_ss(tmem + 128 * ss, smem_desc(qa + off, 16, 1024), smem_desc(ka + off, 16, 1024), ID_S, k > 0);
+            }
+            mma_commit(s_full + 8 * ss);
+            if (last_user(ss, sit)) mma_commit(k_empty + 8 * st);
+            next(sit, ss);
+            return true;
+        };
+        while (pit < i1 && ok) {
+            // S of this pair, and of the next one too if it is the other slot's (a slot's S waits for its own O product)
+            int nit = pit, ns = ps;
+            next(nit, ns);
+            if (sit == pit && ss == ps) ok = issue_s();
+            if (ok && nit < i1 && ns != ps && sit == nit && ss == ns) ok = issue_s();
+            if (!ok) break;
+            const int n = pit - i0, st = n & 1;
+            if (!wait(v_full + 8 * st, (n >> 1) & 1) || !wait(p_full + 8 * ps, done[ps] & 1)) {
+                ok = false;
+                break;
+            }
+            fence_after();
+            const uint32_t va = base + M::V + st * M::TILE;
+#pragma unroll
+            for (int k = 0; k < TC_TN / 16; k++)
+                mma_ts(tmem + 256 + 128 * ps, tmem + 128 * ps + 8 * k, smem_desc(va + k * 2048, M::BLK, 1024), ID_O,
+                       done[ps] > 0 || k > 0);
+            done[ps]++;
+            if (last_user(ps, pit)) mma_commit(v_empty + 8 * st);
+            next(pit, ps);
+        }
+        if (ok) {
+            mma_commit(o_full);
+            mma_commit(o_full + 8);
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (wid == 15) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+int attend_error_flag(int clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_attend_error, sizeof(int)) != cudaSuccess) return -1;
+    if (clear && v) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(g_attend_error, &zero, sizeof(int));
+    }
+    return v ? 1 : 0;
+}
+
+int attend_tc_supported(int D, int dtype) { return (D == 64 || D == 128) && (dtype == KUSH_F16 || dtype == KUSH_BF16); }
+
+int launch_attend_tc(int D, int bits, int P, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream) {
+    const int64_t tiles = (rows * a.G + TC_TM - 1) / TC_TM + a.S;                  // at most one more per sequence
+    if (tiles > 0x7fffffff || a.H > 65535 || a.n_splits > 65535)
+        return set_error(KUSH_ERR_ARG, "attention: %lld row tiles, %d kv heads, %d splits", (long long)tiles, a.H, a.n_splits);
+    return dispatch_fmt(D, bits, P, dtype, [&](auto Dc, auto Bc, auto Pc, auto in) -> int {
+        using IN = decltype(in);
+        if constexpr (Dc.value == 256 || std::is_same_v<IN, float>) {
+            return KUSH_ERR_UNSUPPORTED;
+        } else {
+            auto kern = attend_tc_kernel<Dc.value, Bc.value, Pc.value, IN>;
+            constexpr int smem = TcSmem<Dc.value>::BYTES;
+            const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e != cudaSuccess) return set_error(KUSH_ERR_CUDA, "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+            launch_pdl(kern, dim3(unsigned(tiles), a.H, a.n_splits), dim3(TC_THREADS), size_t(smem), stream, a);
+            return check_launch("attention (tensor cores)");
+        }
+    });
+}
+
+}  // namespace kush
