@@ -27,12 +27,16 @@ constexpr float TC_TAU = 8.0f;
 
 __device__ int g_attend_error = 0;
 
-template <int D>
+template <int D, int BITS>
 struct TcSmem {
+    static constexpr int DC = BITS == 8 ? D : D / 2;
     static constexpr int BLK = 128 * 128;                    // 128 rows x 64 channels of fp16: one swizzled block
     static constexpr int TILE = BLK * (D / 64);
-    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, REF = V + 2 * TILE;       // REF: fp32 [D]
-    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * 16, BYTES = MISC + 16 + 1024;   // + alignment
+    // ring of packed units on their way in: 16 rows of codes, then the key scales and biases (values: 16 of each)
+    static constexpr int SLOT = 16 * DC + 4 * D, NS = D == 64 ? 24 : BITS == 4 ? 20 : 12;
+    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, RING = V + 2 * TILE, REF = RING + NS * SLOT;   // REF: fp32 [D]
+    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * (14 + NS), BROUGHT = MISC + 16, BYTES = BROUGHT + 4 * NS + 1024;   // + alignment
+    static_assert(BYTES <= 232448, "shared memory of a block");
 };
 
 // ------------------------------------------------------------------ tcgen05 / TMEM helpers
@@ -168,7 +172,7 @@ __device__ __forceinline__ void load_words(const uint8_t* p, T* w, int n) {     
     }
 }
 
-// A 16-token unit of a key tile for one warp: lane = (row group rg, column c) holds rows RPL rg .. + RPL - 1, BPL bytes each.
+// A 16-token unit of a key tile for one warp: lane = (row group rg, column c) holds rows rg, rg + RG, ..., BPL bytes each.
 template <int D, int BITS, int P>
 struct Unit {
     using F = Fmt<D, BITS, P>;
@@ -178,12 +182,36 @@ struct Unit {
     __device__ static int hi_chunk(int c) { return BITS == 4 ? c + D / 16 : 2 * c + 1; }
 };
 
+// one thread: an untiled bulk copy into shared memory, completing on `bar` (16-byte addresses and size; no multicast)
+__device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_done(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // grid (row tiles, Hkv, n_splits), block 512
 template <int D, int BITS, int P, class IN>
 __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) {
     using F = Fmt<D, BITS, P>;
     using U = Unit<D, BITS, P>;
-    using M = TcSmem<D>;
+    using M = TcSmem<D, BITS>;
     constexpr int CH = D / 8;                                      // 8-channel chunks of a row
     extern __shared__ uint8_t smem_raw[];
     pdl_wait();
@@ -210,31 +238,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     float* ref = reinterpret_cast<float*>(sm + M::REF);
     const uint32_t bars = base + M::BARS;
     const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64,
-                   p_full = bars + 80, o_full = bars + 96;                         // pairs: [stage] or [slot]
+                   p_full = bars + 80, o_full = bars + 96, r_full = bars + 112;    // pairs: [stage] or [slot]; [ring]
     volatile int* gave_up = reinterpret_cast<volatile int*>(sm + M::MISC);
+    volatile int* brought = reinterpret_cast<volatile int*>(sm + M::BROUGHT);    // [ring] the unit last brought to a slot
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + M::MISC + 4);
     if (tid == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(sm + M::BARS);
         const int count[7] = {8, 1, 8, 1, 1, 4, 1};
-        for (int i = 0; i < 14; i++) mbar_init(b + i, count[i / 2]);
+        for (int i = 0; i < 14 + M::NS; i++) mbar_init(b + i, i < 14 ? count[i / 2] : 1);
         *gave_up = 0;
+        for (int i = 0; i < M::NS; i++) brought[i] = -1;
         fence_mbar_init();
     }
     if (wid == 15) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    // bounded wait; false if this block gave up
-    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    // bounded wait for a condition; false if this block gave up
+    auto until = [&](auto ready) -> bool {
         uint64_t t0 = 0;
         for (uint32_t n = 0;; n++) {
-            uint32_t ok;
-            asm volatile(
-                "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                : "=r"(ok)
-                : "r"(bar), "r"(parity)
-                : "memory");
-            if (ok) return true;
+            if (ready()) return true;
             if (*gave_up) return false;
             if (n % 64 == 0) {
                 uint64_t now;
@@ -248,6 +272,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             }
         }
     };
+    // for the phase of `parity` of a barrier
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return until([&] { return mbar_done(bar, parity); }); };
     const int32_t* bt = a.block_table + int64_t(t.s) * a.max_pages;
     const uint8_t* hcache = a.cache + int64_t(h) * a.head_stride;
     const int full = t.ctx / P * P;                                                // cached tokens in finished pages
@@ -277,15 +303,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_at;
-    // slot i's rows' positions, and whether it works on the key tile of index i
-    auto slot_p0 = [&](int i) { return paired && i == 1 ? t.ctx + (t.r0 + 128) / a.G : t.p0; };
-    auto slot_p1 = [&](int i) { return paired && i == 0 ? t.ctx + (t.r0 + 127) / a.G : t.p1; };
+    // whether slot i works on the key tile of index it: paired, some row of the slot sees a token of it
+    const int mid0 = t.ctx + (t.r0 + 127) / a.G, mid1 = t.ctx + (t.r0 + 128) / a.G;    // last row of slot 0, first of slot 1
+    const int lo1 = a.window > 0 ? max(0, mid1 - a.window + 1) : 0;
     auto active = [&](int slot, int it) -> bool {
         if (!paired) return ((it - i0) & 1) == slot;
         const int j0 = kt.tile(it) * TC_TN;
-        if (j0 > slot_p1(slot)) return false;
-        const int lo = a.window > 0 ? max(0, slot_p0(slot) - a.window + 1) : 0;
-        return j0 + TC_TN > lo || j0 < a.sinks;
+        return slot == 0 ? j0 <= mid0 : j0 + TC_TN > lo1 || j0 < a.sinks;
     };
     bool ok = true;
 
@@ -303,38 +327,40 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         int n = 0;                                                                 // tiles done by this slot
         for (int it = i0; it < i1; it++) {
             if (!active(slot, it)) continue;
-            if (!wait(s_full + 8 * slot, n & 1)) {
-                ok = false;
-                break;
-            }
+            ok = __all_sync(0xffffffffu, wait(s_full + 8 * slot, n & 1));           // (converged: tcgen05.ld is warp-aligned)
+            if (!ok) break;
             fence_after();
             if (busy) {
                 const int j0 = kt.tile(it) * TC_TN;
                 // columns [0, hi] seen, and of those [lo, ...) or [0, sk)
                 const int hi = pos - j0, lo = a.window > 0 ? pos - a.window + 1 - j0 : -1, sk = a.sinks - j0;
                 const bool cut = j0 + TC_TN - 1 > wp0 || (a.window > 0 && j0 < wp1 - a.window + 1 && j0 + TC_TN > a.sinks);
-                auto load = [&](int c, uint32_t (&x)[32]) {
-                    tmem_ld32(s_at + 32 * c, x);
-                    wait_ld();
-                    if (cut) {
+                // (loops over 32-column pieces stay rolled: five roles' code shares the instruction caches)
+                if (cut) {                                                         // masked scores become -inf in TMEM
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t x[32];
+                        tmem_ld32(s_at + 32 * c, x);
+                        wait_ld();
+                        const int h0 = hi - 32 * c, l0 = lo - 32 * c, k0 = sk - 32 * c;
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const int col = 32 * c + i;
-                            if (col > hi || (col < lo && col >= sk)) x[i] = 0xFF800000u;      // -inf
-                        }
+                        for (int i = 0; i < 32; i++)
+                            if (i > h0 || (i < l0 && i >= k0)) x[i] = 0xFF800000u;
+                        tmem_st32(s_at + 32 * c, x);
                     }
-                };
+                    wait_st();
+                }
                 float mx = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
+                    uint32_t x[32], y[32];
+                    tmem_ld32(s_at + 32 * c, x);
+                    tmem_ld32(s_at + 32 * c + 32, y);
+                    wait_ld();
+                    float m4[4] = {mx, mx, mx, mx};
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t x[32];
-                    load(c, x);
-                    float m4[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) m4[i] = __uint_as_float(x[i]);
-#pragma unroll
-                    for (int i = 4; i < 32; i++) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(x[i]));
-                    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                    for (int i = 0; i < 32; i++) m4[i & 3] = max3(m4[i & 3], __uint_as_float(x[i]), __uint_as_float(y[i]));
+                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
                 mx *= sc;
                 const bool bump = mx > m + TC_TAU;                                 // (m = -inf: any score)
@@ -344,7 +370,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     m = mn;
                     l *= corr;
                     if (n > 0) {                                                   // the slot's last product is done
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t x[32];
                             tmem_ld32(o_at + 32 * c, x);
@@ -356,22 +382,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     }
                 }
                 const float mm = m == -INFINITY ? 0.0f : m;                        // nothing seen yet: weights 0
-                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
+                const float2 sc2 = make_float2(sc, sc), mm2 = make_float2(-mm, -mm);
+                float2 la = make_float2(0.0f, 0.0f), lb = la;
+#pragma unroll 1
                 for (int c = 0; c < 4; c++) {
                     uint32_t x[32], p[16];
-                    load(c, x);
+                    tmem_ld32(s_at + 32 * c, x);
+                    wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float e0 = ex2(fmaf(__uint_as_float(x[2 * i]), sc, -mm));
-                        const float e1 = ex2(fmaf(__uint_as_float(x[2 * i + 1]), sc, -mm));
-                        l4[i & 1] += e0;
-                        l4[2 + (i & 1)] += e1;
-                        p[i] = h2_pack(e0, e1);
+                        const float2 d = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc2, mm2);
+                        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+                        if (i & 1) lb = __fadd2_rn(lb, e);
+                        else la = __fadd2_rn(la, e);
+                        p[i] = h2_pack(e.x, e.y);
                     }
                     tmem_st16(s_at + 16 * c, p);
                 }
-                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                l += (la.x + la.y) + (lb.x + lb.y);
                 wait_st();
             }
             fence_before();
@@ -381,7 +409,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         }
         // ---------------------------------------------------------------- the slot's output
         if (ok && n > 0) {
-            ok = wait(o_full + 8 * slot, 0);
+            ok = __all_sync(0xffffffffu, wait(o_full + 8 * slot, 0));
             fence_after();
         }
         // split: slot 1 hands its maximum, sum and output over (in the key buffers, no longer read)
@@ -389,7 +417,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         float* xo = xm + 256;                                                      // [128][D + 4]
         if (!paired) {
             // both slots' products are done before the key buffers are reused
-            if (ok && slot == 1 && i1 - i0 > 0) ok = wait(o_full, 0);
+            if (ok && slot == 1) ok = __all_sync(0xffffffffu, wait(o_full, 0));
             if (slot == 1 && busy) {
                 xm[row] = n > 0 ? m : -INFINITY;
                 xm[128 + row] = l;
@@ -473,109 +501,175 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             rf[i] = h2_pack(ref[8 * lo_c + 2 * i], ref[8 * lo_c + 2 * i + 1]);
             rf[4 + i] = h2_pack(ref[8 * hi_c + 2 * i], ref[8 * hi_c + 2 * i + 1]);
         }
-        // the stream of units: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp takes every 7th
-        auto fill = [&](auto kvc, int n, int u) {
+        // The stream of units x: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp converts every 7th.
+        // Packed units come through a ring of NS slots, in stream order; whoever has converted unit x brings x + NS into
+        // its slot (units that are not packed only complete the slot's phase).
+        const int units = 16 * (i1 - i0);
+        auto first_token = [&](int x) { return kt.tile(i0 + (x >> 4)) * TC_TN + 16 * (x & 7); };
+        auto kind_of = [&](int j0) {                                               // 0 unseen, 1 packed, 2 new rows, 3 mixed
+            if (j0 > t.p1 || (j0 + 15 < kt.lo && j0 >= kt.ns)) return 0;
+            return j0 + 16 <= full ? 1 : j0 >= t.ctx && j0 + 15 <= t.p1 ? 2 : 3;
+        };
+        auto block_of = [&](int x) -> int32_t {                                    // block id of a packed unit
+            if (x >= units) return 0;
+            const int j0 = first_token(x);
+            return kind_of(j0) == 1 ? bt[j0 / P] : 0;
+        };
+        auto bring = [&](int x, int32_t blk) {
+            if (x >= units || lane != 0) return;
+            const int slot = x % M::NS, j0 = first_token(x);
+            const uint32_t bar = r_full + 8 * slot, dst = base + M::RING + slot * M::SLOT;
+            // x - NS has landed and is converted.  The slot is marked after this phase's one arrival: who sees the mark may
+            // bring x + NS, whose arrival must find this phase closed.
+            if (kind_of(j0) != 1) {
+                bar_arrive(bar);
+                brought[slot] = x;
+                return;
+            }
+            const uint8_t* rec = hcache + int64_t(blk) * a.block_stride;
+            const int r0 = j0 % P;
+            if (x & 8) {
+                bar_expect(bar, 16 * F::DC + 64);
+                brought[slot] = x;
+                bulk_in(dst, rec + F::OFF_VQ + r0 * F::DC, 16 * F::DC, bar);
+                if constexpr (P == 16) {
+                    bulk_in(dst + 16 * F::DC, rec + F::OFF_VS, 64, bar);           // scales, then biases
+                } else {
+                    bulk_in(dst + 16 * F::DC, rec + F::OFF_VS + 2 * r0, 32, bar);
+                    bulk_in(dst + 16 * F::DC + 32, rec + F::OFF_VB + 2 * r0, 32, bar);
+                }
+            } else {
+                bar_expect(bar, 16 * F::DC + 4 * D);
+                brought[slot] = x;
+                bulk_in(dst, rec + r0 * F::DC, 16 * F::DC, bar);
+                bulk_in(dst + 16 * F::DC, rec + F::OFF_KS, 4 * D, bar);
+            }
+        };
+        // A warp may be ahead of the one that converts x - NS and then brings x: a parity alone does not tell x's phase from
+        // the one two before it, so the slot says first which unit was brought.
+        auto was_brought = [&](int x) -> bool { return until([&] { return brought[x % M::NS] == x; }); };
+        auto fill = [&](auto kvc, int x) {
             constexpr bool kv = decltype(kvc)::value;                              // values (else keys)
-            const int st = n & 1;
-            const int j0 = kt.tile(i0 + n) * TC_TN + 16 * u;                       // the unit's first token
-            const bool none = j0 > t.p1 || (j0 + 15 < kt.lo && j0 >= kt.ns);       // no row sees a token of it
-            const int kind = none ? 0 : j0 + 16 <= full ? 1 : j0 >= t.ctx && j0 + 15 <= t.p1 ? 2 : 3;
+            const int n = x >> 4, u = x & 7, st = n & 1;
+            const int j0 = first_token(x), kind = kind_of(j0);
             const uint32_t dst = base + (kv ? M::V : M::K) + st * M::TILE;
             const uint32_t bar_e = (kv ? v_empty : k_empty) + 8 * st, bar_f = (kv ? v_full : k_full) + 8 * st;
             if (kind == 1) {
-                const uint8_t* rec = hcache + int64_t(bt[j0 / P]) * a.block_stride;
-                const int row0 = j0 % P + U::RPL * rg;
-                uint32_t w[U::RPL][U::W];
-#pragma unroll
-                for (int i = 0; i < U::RPL; i++)
-                    load_words(rec + (kv ? F::OFF_VQ : 0) + (row0 + i) * F::DC + U::BPL * c, w[i], U::W);
+                const uint8_t* raw = sm + M::RING + (x % M::NS) * M::SLOT;
+                if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
+                if (!was_brought(x) || !wait(r_full + 8 * (x % M::NS), (x / M::NS) & 1)) ok = false;
                 uint32_t s[8], b[8];
                 if constexpr (!kv) {
-                    load_words(rec + F::OFF_KS + 16 * lo_c, s, 4);
-                    load_words(rec + F::OFF_KS + 16 * hi_c, s + 4, 4);
-                    load_words(rec + F::OFF_KB + 16 * lo_c, b, 4);
-                    load_words(rec + F::OFF_KB + 16 * hi_c, b + 4, 4);
+                    load_words(raw + 16 * F::DC + 16 * lo_c, s, 4);
+                    load_words(raw + 16 * F::DC + 16 * hi_c, s + 4, 4);
+                    load_words(raw + 16 * F::DC + 2 * D + 16 * lo_c, b, 4);
+                    load_words(raw + 16 * F::DC + 2 * D + 16 * hi_c, b + 4, 4);
 #pragma unroll
                     for (int i = 0; i < 8; i++) b[i] = h2_sub_u(b[i], rf[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < U::RPL; i++) {
-                        s[i] = uint32_t(reinterpret_cast<const uint16_t*>(rec + F::OFF_VS)[row0 + i]) * 0x10001u;
-                        b[i] = uint32_t(reinterpret_cast<const uint16_t*>(rec + F::OFF_VB)[row0 + i]) * 0x10001u;
-                    }
                 }
-                if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
-#pragma unroll
+#pragma unroll 2
                 for (int i = 0; i < U::RPL; i++) {
-                    uint32_t lo[4], hi[4];
-                    codes_of<BITS>(w[i], lo, hi);
+                    const int row = rg + U::RG * i;
+                    uint32_t w[U::W], lo[4], hi[4];
+                    load_words(raw + row * F::DC + U::BPL * c, w, U::W);
+                    codes_of<BITS>(w, lo, hi);
+                    if constexpr (kv) {
+                        const uint32_t vs = uint32_t(reinterpret_cast<const uint16_t*>(raw + 16 * F::DC)[row]) * 0x10001u;
+                        const uint32_t vb = uint32_t(reinterpret_cast<const uint16_t*>(raw + 16 * F::DC + 32)[row]) * 0x10001u;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        lo[j] = h2_fma_u(lo[j], kv ? s[i] : s[j], kv ? b[i] : b[j]);
-                        hi[j] = h2_fma_u(hi[j], kv ? s[i] : s[4 + j], kv ? b[i] : b[4 + j]);
-                    }
-                    const int row = 16 * u + U::RPL * rg + i;
-                    if (flip) {
-                        st_chunk(dst + tile_off(row, hi_c), hi[0], hi[1], hi[2], hi[3]);
-                        st_chunk(dst + tile_off(row, lo_c), lo[0], lo[1], lo[2], lo[3]);
+                        for (int j = 0; j < 4; j++) {
+                            lo[j] = h2_fma_u(lo[j], vs, vb);
+                            hi[j] = h2_fma_u(hi[j], vs, vb);
+                        }
                     } else {
-                        st_chunk(dst + tile_off(row, lo_c), lo[0], lo[1], lo[2], lo[3]);
-                        st_chunk(dst + tile_off(row, hi_c), hi[0], hi[1], hi[2], hi[3]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            lo[j] = h2_fma_u(lo[j], s[j], b[j]);
+                            hi[j] = h2_fma_u(hi[j], s[4 + j], b[4 + j]);
+                        }
                     }
+                    const uint32_t at_lo = dst + tile_off(16 * u + row, lo_c), at_hi = dst + tile_off(16 * u + row, hi_c);
+                    st_chunk(flip ? at_hi : at_lo, flip ? hi[0] : lo[0], flip ? hi[1] : lo[1], flip ? hi[2] : lo[2], flip ? hi[3] : lo[3]);
+                    st_chunk(flip ? at_lo : at_hi, flip ? lo[0] : hi[0], flip ? lo[1] : hi[1], flip ? lo[2] : hi[2], flip ? lo[3] : hi[3]);
                 }
             } else {
                 // new rows, the unfinished page, unseen tokens: 8-channel chunks of a row, CH lanes per row
                 constexpr int RPI = WARP / CH, NI = 16 / RPI;                      // rows per step, steps
-                const int cc = lane % CH;
+                const int cc = lane % CH, r0 = lane / CH;
                 uint4 raw[NI];
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
-                    const int j = j0 + i * RPI + lane / CH;
+                    const int j = j0 + i * RPI + r0;
+                    const bool see = kind == 2 || (kind == 3 && kt.seen(j, t.p1));
                     raw[i] = make_uint4(0, 0, 0, 0);
-                    if (kind == 2 || (kind == 3 && kt.seen(j, t.p1) && j >= t.ctx)) {
+                    if (see && j >= t.ctx) {
                         const IN* src = kv ? vn + int64_t(j - t.ctx) * a.v_stride : kn + int64_t(j - t.ctx) * a.k_stride;
                         raw[i] = *reinterpret_cast<const uint4*>(src + 8 * cc);
-                    } else if (!kv && kind == 3 && kt.seen(j, t.p1) && j >= full) {
+                    } else if (!kv && see && j >= full) {
                         raw[i] = *reinterpret_cast<const uint4*>(tail + (j % P) * D + 8 * cc);
                     }
+                }
+                float rf8[8];
+                if constexpr (!kv) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) rf8[k] = ref[8 * cc + k];
                 }
                 if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
-                    const int row = 16 * u + i * RPI + lane / CH, j = j0 + i * RPI + lane / CH;
+                    const int row = 16 * u + i * RPI + r0, j = j0 + i * RPI + r0;
                     const IN* e = reinterpret_cast<const IN*>(&raw[i]);
-                    float x[8];
+                    const bool sub = kind == 2 || (kind == 3 && kt.seen(j, t.p1));
+                    uint32_t p[4];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] = to_f32(e[k]);
-                    const bool see = kind == 2 || (kind == 3 && kt.seen(j, t.p1));
-                    if (kind == 3 && see && j < t.ctx && (kv || j < full)) {       // from a record, one by one
+                    for (int k = 0; k < 4; k++)
+                        p[k] = kv || !sub ? h2_pack(to_f32(e[2 * k]), to_f32(e[2 * k + 1]))
+                                          : h2_pack(to_f32(e[2 * k]) - rf8[2 * k], to_f32(e[2 * k + 1]) - rf8[2 * k + 1]);
+                    st_chunk(dst + tile_off(row, cc), p[0], p[1], p[2], p[3]);
+                }
+                if (kind == 3) {                                                   // its cached tokens, one row after the other
+#pragma unroll 1
+                    for (int i = 0; i < NI; i++) {
+                        const int row = 16 * u + i * RPI + r0, j = j0 + i * RPI + r0;
+                        if (!kt.seen(j, t.p1) || j >= (kv ? t.ctx : full)) continue;
                         const uint8_t* rec = hcache + int64_t(bt[j / P]) * a.block_stride;
-                        const int s = j % P;
+                        const int at = j % P;
+                        float y[8];
 #pragma unroll
                         for (int k = 0; k < 8; k++) {
                             const int d = 8 * cc + k;
-                            x[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + s * F::DC, d)), h_load(rec + F::OFF_VS, s),
-                                             h_load(rec + F::OFF_VB, s))
-                                      : fmaf(float(code_at<D, BITS>(rec + s * F::DC, d)), h_load(rec + F::OFF_KS, d),
-                                             h_load(rec + F::OFF_KB, d));
+                            y[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + at * F::DC, d)), h_load(rec + F::OFF_VS, at),
+                                             h_load(rec + F::OFF_VB, at))
+                                      : fmaf(float(code_at<D, BITS>(rec + at * F::DC, d)), h_load(rec + F::OFF_KS, d),
+                                             h_load(rec + F::OFF_KB, d)) - ref[d];
                         }
+                        st_chunk(dst + tile_off(row, cc), h2_pack(y[0], y[1]), h2_pack(y[2], y[3]), h2_pack(y[4], y[5]),
+                                 h2_pack(y[6], y[7]));
                     }
-                    if (!kv && see) {
-#pragma unroll
-                        for (int k = 0; k < 8; k++) x[k] -= ref[8 * cc + k];
-                    }
-                    st_chunk(dst + tile_off(row, cc), h2_pack(x[0], x[1]), h2_pack(x[2], x[3]), h2_pack(x[4], x[5]),
-                             h2_pack(x[6], x[7]));
                 }
             }
             fence_async();
             __syncwarp();
             if (lane == 0) bar_arrive(bar_f);
         };
-        for (int x = wid - 8; x < 16 * (i1 - i0) && ok; x += TC_NPROD) {
-            if (x & 8) fill(IC<1>{}, x >> 4, x & 7);
-            else fill(IC<0>{}, x >> 4, x & 7);
+        for (int x = wid - 8; x < M::NS; x += TC_NPROD) bring(x, block_of(x));
+        int x = wid - 8;
+        for (; x < units && ok; x += TC_NPROD) {
+            const int32_t blk = block_of(x + M::NS);
+            if (x & 8) fill(IC<1>{}, x);
+            else fill(IC<0>{}, x);
             ok = __all_sync(0xffffffffu, ok);
+            if (ok && was_brought(x)) bring(x + M::NS, blk);                       // (units of a slot are brought in order)
+        }
+        if (!ok) {
+            // given up: a bounded wait for the copies that this warp has issued and that may still be in flight
+            auto landed = [&](int y) {
+                if (y >= units || kind_of(first_token(y)) != 1) return;
+                for (int i = 0; i < 1 << 16 && !mbar_done(r_full + 8 * (y % M::NS), (y / M::NS) & 1); i++) {
+                }
+            };
+            for (int y = wid - 8; y < M::NS; y += TC_NPROD) landed(y);
+            for (int y = x - TC_NPROD; y >= max(0, x - TC_NPROD - M::NS); y -= TC_NPROD) landed(y + M::NS);
         }
     } else if (lane == 0) {
         // ---------------------------------------------------------------- the products, in the order of (tile, slot)
@@ -630,9 +724,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             if (last_user(ps, pit)) mma_commit(v_empty + 8 * st);
             next(pit, ps);
         }
-        if (ok) {
-            mma_commit(o_full);
-            mma_commit(o_full + 8);
+        // both slots' outputs; nothing of this block is in flight when it ends, whatever ended the loop
+        mma_commit(o_full);
+        mma_commit(o_full + 8);
+        for (int i = 0; i < 1 << 20 && !(mbar_done(o_full, 0) && mbar_done(o_full + 8, 0)); i++) {
         }
     }
     __syncwarp();
@@ -665,7 +760,7 @@ int launch_attend_tc(int D, int bits, int P, int dtype, const AttendArgs& a, int
             return KUSH_ERR_UNSUPPORTED;
         } else {
             auto kern = attend_tc_kernel<Dc.value, Bc.value, Pc.value, IN>;
-            constexpr int smem = TcSmem<Dc.value>::BYTES;
+            constexpr int smem = TcSmem<Dc.value, Bc.value>::BYTES;
             const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
             if (e != cudaSuccess) return set_error(KUSH_ERR_CUDA, "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
             launch_pdl(kern, dim3(unsigned(tiles), a.H, a.n_splits), dim3(TC_THREADS), size_t(smem), stream, a);
