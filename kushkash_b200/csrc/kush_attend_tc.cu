@@ -303,13 +303,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_at;
-    // whether slot i works on the key tile of index it: paired, some row of the slot sees a token of it
-    const int mid0 = t.ctx + (t.r0 + 127) / a.G, mid1 = t.ctx + (t.r0 + 128) / a.G;    // last row of slot 0, first of slot 1
-    const int lo1 = a.window > 0 ? max(0, mid1 - a.window + 1) : 0;
+    // Whether a slot works on the key tile of index it.  Split: in turn.  Paired: some row of the slot sees a token of it:
+    // slot 0 (whose last row is mid0) the tiles up to end0, slot 1 (whose first row is mid0 or mid0 + 1) all but the window
+    // tiles [gap0, gap1) behind the sinks that only slot 0's rows reach back to.
+    int end0 = i1, gap0 = 0, gap1 = 0;
+    if (paired) {
+        const int mid0 = t.ctx + (t.r0 + 127) / a.G, mid1 = t.ctx + (t.r0 + 128) / a.G;
+        const int lo1 = a.window > 0 ? max(0, mid1 - a.window + 1) : 0;
+        end0 = min(i1, kt.a + mid0 / TC_TN + 1 - kt.b);                            // (mid0 >= lo: a window tile)
+        gap0 = kt.a + (a.sinks > kt.b * TC_TN ? (min(a.sinks, lo1) + TC_TN - 1) / TC_TN - kt.b : 0);
+        gap1 = kt.a + lo1 / TC_TN - kt.b;                                          // (lo1 <= mid1, a tile of the list)
+    }
     auto active = [&](int slot, int it) -> bool {
         if (!paired) return ((it - i0) & 1) == slot;
-        const int j0 = kt.tile(it) * TC_TN;
-        return slot == 0 ? j0 <= mid0 : j0 + TC_TN > lo1 || j0 < a.sinks;
+        return slot == 0 ? it < end0 : it < gap0 || it >= gap1;
     };
     bool ok = true;
 
@@ -673,56 +680,57 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         }
     } else if (lane == 0) {
         // ---------------------------------------------------------------- the products, in the order of (tile, slot)
+        // S of a pair goes out before O of the pair before it when the slots differ, so that one slot's softmax runs under
+        // the other's products; a slot's own S has to wait for its O product, which reads P from S's columns.
         constexpr uint32_t ID_S = instr_desc(128, TC_TN, false), ID_O = instr_desc(128, D, true);
-        auto next = [&](int& it, int& slot) {                                      // the next active (tile, slot) pair
-            do {
-                if (++slot == 2) {
-                    slot = 0;
-                    it++;
-                }
-            } while (it < i1 && !active(slot, it));
-        };
-        auto last_user = [&](int slot, int it) { return slot == 1 || !active(1, it); };
-        int sit = i0, ss = -1, pit = i0, ps = -1;                                  // cursors of S and of O products
-        next(sit, ss);
-        next(pit, ps);
+        const uint64_t q_desc = smem_desc(base + M::Q, 16, 1024), k_desc = smem_desc(base + M::K, 16, 1024);
+        const uint64_t v_desc = smem_desc(base + M::V, M::BLK, 1024);
         uint32_t done[2] = {0, 0};                                                 // O products issued per slot
-        auto issue_s = [&]() -> bool {
-            const int n = sit - i0, st = n & 1;
-            if (!wait(k_full + 8 * st, (n >> 1) & 1)) return false;
-            fence_after();
-            const uint32_t qa = base + M::Q + (paired && ss == 1 ? M::TILE : 0), ka = base + M::K + st * M::TILE;
+        int pit = -1, ps = 0;                                                      // the pair whose O product is due
+        int it = i0, slot = active(0, i0) ? 0 : 1;
+        while (ok && (it < i1 || pit >= 0)) {
+            const bool more = it < i1, s_first = pit < 0 || (more && slot != ps);
+#pragma unroll 1
+            for (int step = 0; step < 2 && ok; step++) {
+                if ((step == 0) == s_first) {
+                    if (!more) continue;
+                    const int n = it - i0, st = n & 1;
+                    ok = wait(k_full + 8 * st, (n >> 1) & 1);
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t qd = q_desc + (paired && slot ? M::TILE >> 4 : 0), kd = k_desc + st * (M::TILE >> 4);
 #pragma unroll
-            for (int k = 0; k < D / 16; k++) {
-                const uint32_t off = (k >> 2) * M::BLK + (k & 3) * 32;
-                mma_ss(tmem + 128 * ss, smem_desc(qa + off, 16, 1024), smem_desc(ka + off, 16, 1024), ID_S, k > 0);
-            }
-            mma_commit(s_full + 8 * ss);
-            if (last_user(ss, sit)) mma_commit(k_empty + 8 * st);
-            next(sit, ss);
-            return true;
-        };
-        while (pit < i1 && ok) {
-            // S of this pair, and of the next one too if it is the other slot's (a slot's S waits for its own O product)
-            int nit = pit, ns = ps;
-            next(nit, ns);
-            if (sit == pit && ss == ps) ok = issue_s();
-            if (ok && nit < i1 && ns != ps && sit == nit && ss == ns) ok = issue_s();
-            if (!ok) break;
-            const int n = pit - i0, st = n & 1;
-            if (!wait(v_full + 8 * st, (n >> 1) & 1) || !wait(p_full + 8 * ps, done[ps] & 1)) {
-                ok = false;
-                break;
-            }
-            fence_after();
-            const uint32_t va = base + M::V + st * M::TILE;
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint32_t off = ((k >> 2) * M::BLK + (k & 3) * 32) >> 4;
+                        mma_ss(tmem + 128 * slot, qd + off, kd + off, ID_S, k > 0);
+                    }
+                    mma_commit(s_full + 8 * slot);
+                    if (slot == 1 || !active(1, it)) mma_commit(k_empty + 8 * st);
+                } else if (pit >= 0) {
+                    const int n = pit - i0, st = n & 1;
+                    ok = wait(v_full + 8 * st, (n >> 1) & 1) && wait(p_full + 8 * ps, (ps ? done[1] : done[0]) & 1);
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t vd = v_desc + st * (M::TILE >> 4);
+                    const bool acc = (ps ? done[1] : done[0]) > 0;
 #pragma unroll
-            for (int k = 0; k < TC_TN / 16; k++)
-                mma_ts(tmem + 256 + 128 * ps, tmem + 128 * ps + 8 * k, smem_desc(va + k * 2048, M::BLK, 1024), ID_O,
-                       done[ps] > 0 || k > 0);
-            done[ps]++;
-            if (last_user(ps, pit)) mma_commit(v_empty + 8 * st);
-            next(pit, ps);
+                    for (int k = 0; k < TC_TN / 16; k++)
+                        mma_ts(tmem + 256 + 128 * ps, tmem + 128 * ps + 8 * k, vd + k * (2048 >> 4), ID_O, acc || k > 0);
+                    if (ps) done[1]++;
+                    else done[0]++;
+                    if (ps == 1 || !active(1, pit)) mma_commit(v_empty + 8 * st);
+                }
+            }
+            pit = more ? it : -1;
+            ps = slot;
+            if (more) {                                                            // the next active pair
+                if (slot == 0 && active(1, it)) {
+                    slot = 1;
+                } else {
+                    it++;
+                    slot = it < i1 && active(0, it) ? 0 : 1;
+                }
+            }
         }
         // both slots' outputs; nothing of this block is in flight when it ends, whatever ended the loop
         mma_commit(o_full);
