@@ -177,9 +177,6 @@ template <int D, int BITS, int P>
 struct Unit {
     using F = Fmt<D, BITS, P>;
     static constexpr int W = BITS / 2, BPL = 4 * W, LPR = F::DC / BPL, RG = WARP / LPR, RPL = 16 / RG;
-    // first chunks (8 channels) of the lane's lo and hi halves
-    __device__ static int lo_chunk(int c) { return BITS == 4 ? c : 2 * c; }
-    __device__ static int hi_chunk(int c) { return BITS == 4 ? c + D / 16 : 2 * c + 1; }
 };
 
 // one thread: an untiled bulk copy into shared memory, completing on `bar` (16-byte addresses and size; no multicast)
@@ -190,6 +187,11 @@ __device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t 
 }
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ bool mbar_done(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -500,14 +502,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         const IN* tail = static_cast<const IN*>(a.tail_k) + (int64_t(a.tail_idx[t.s]) * a.H + h) * P * D;
         const IN* kn = static_cast<const IN*>(a.k_new) + t.q0 * a.k_stride + int64_t(h) * D;
         const IN* vn = static_cast<const IN*>(a.v_new) + t.q0 * a.v_stride + int64_t(h) * D;
-        const int lo_c = U::lo_chunk(c), hi_c = U::hi_chunk(c);
-        const bool flip = BITS == 8 ? (c >> 2) & 1 : D == 64 && (rg & 1);          // store order: spread the banks
+        // the lane's two chunks, in the order of its stores (int8: lanes of a row's second block store their odd chunk
+        // first, so that the eight lanes of a row fall in distinct banks)
+        const int swap = BITS == 8 && D == 128 ? c >> 2 : 0;
+        const int c_a = BITS == 4 ? c : 2 * c + swap, c_b = BITS == 4 ? c + D / 16 : 2 * c + 1 - swap;
+        const uint32_t at_a = tile_off(rg, c_a), at_b = tile_off(rg, c_b);         // in a unit's first rows
         uint32_t rf[8];                                                            // the reference of the lane's channels
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            rf[i] = h2_pack(ref[8 * lo_c + 2 * i], ref[8 * lo_c + 2 * i + 1]);
-            rf[4 + i] = h2_pack(ref[8 * hi_c + 2 * i], ref[8 * hi_c + 2 * i + 1]);
+            rf[i] = h2_pack(ref[8 * c_a + 2 * i], ref[8 * c_a + 2 * i + 1]);
+            rf[4 + i] = h2_pack(ref[8 * c_b + 2 * i], ref[8 * c_b + 2 * i + 1]);
         }
+        constexpr int RPI = WARP / CH, NI = 16 / RPI;                              // unpacked rows: rows per step, steps
+        const int cc = lane % CH, r0 = lane / CH;
+        float rf8[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) rf8[k] = ref[8 * cc + k];
         // The stream of units x: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp converts every 7th.
         // Packed units come through a ring of NS slots, in stream order; whoever has converted unit x brings x + NS into
         // its slot (units that are not packed only complete the slot's phase).
@@ -554,90 +564,105 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         };
         // A warp may be ahead of the one that converts x - NS and then brings x: a parity alone does not tell x's phase from
         // the one two before it, so the slot says first which unit was brought.
-        auto was_brought = [&](int x) -> bool { return until([&] { return brought[x % M::NS] == x; }); };
-        auto fill = [&](auto kvc, int x) {
+        auto was_brought = [&](int x, int slot) -> bool { return until([&] { return brought[slot] == x; }); };
+        // a row of an unpacked unit (new rows, the unfinished page, unseen tokens): 16 bytes of row i * RPI + r0
+        auto unpacked = [&](bool kv, int j0, int kind, int i) -> uint4 {
+            const int j = j0 + i * RPI + r0;
+            const IN* src = nullptr;
+            if (kind == 2 || (kind == 3 && j >= t.ctx && kt.seen(j, t.p1)))
+                src = kv ? vn + int64_t(j - t.ctx) * a.v_stride : kn + int64_t(j - t.ctx) * a.k_stride;
+            else if (kind == 3 && !kv && j >= full && kt.seen(j, t.p1))
+                src = tail + (j % P) * D;
+            return src ? *reinterpret_cast<const uint4*>(src + 8 * cc) : make_uint4(0, 0, 0, 0);
+        };
+        uint4 raw[NI];                                                             // this warp's next unpacked unit
+        auto packed_unit = [&](auto kvc, int x, uint32_t dst, int slot) {
             constexpr bool kv = decltype(kvc)::value;                              // values (else keys)
-            const int n = x >> 4, u = x & 7, st = n & 1;
-            const int j0 = first_token(x), kind = kind_of(j0);
-            const uint32_t dst = base + (kv ? M::V : M::K) + st * M::TILE;
-            const uint32_t bar_e = (kv ? v_empty : k_empty) + 8 * st, bar_f = (kv ? v_full : k_full) + 8 * st;
-            if (kind == 1) {
-                const uint8_t* raw = sm + M::RING + (x % M::NS) * M::SLOT;
-                if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
-                if (!was_brought(x) || !wait(r_full + 8 * (x % M::NS), (x / M::NS) & 1)) ok = false;
-                uint32_t s[8], b[8];
-                if constexpr (!kv) {
-                    load_words(raw + 16 * F::DC + 16 * lo_c, s, 4);
-                    load_words(raw + 16 * F::DC + 16 * hi_c, s + 4, 4);
-                    load_words(raw + 16 * F::DC + 2 * D + 16 * lo_c, b, 4);
-                    load_words(raw + 16 * F::DC + 2 * D + 16 * hi_c, b + 4, 4);
+            const uint8_t* u8 = sm + M::RING + slot * M::SLOT;
+            uint32_t s[8], b[8];
+            if constexpr (!kv) {
+                load_words(u8 + 16 * F::DC + 16 * c_a, s, 4);
+                load_words(u8 + 16 * F::DC + 16 * c_b, s + 4, 4);
+                load_words(u8 + 16 * F::DC + 2 * D + 16 * c_a, b, 4);
+                load_words(u8 + 16 * F::DC + 2 * D + 16 * c_b, b + 4, 4);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) b[i] = h2_sub_u(b[i], rf[i]);
+                for (int i = 0; i < 8; i++) b[i] = h2_sub_u(b[i], rf[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < U::RPL; i++) {
+                const int row = rg + U::RG * i;
+                uint32_t w[U::W], lo[4], hi[4];
+                if constexpr (BITS == 4) {
+                    load_words(u8 + row * F::DC + 8 * c, w, 2);
+                } else {
+                    load_words(u8 + row * F::DC + 8 * c_a, w, 2);
+                    load_words(u8 + row * F::DC + 8 * c_b, w + 2, 2);
                 }
-#pragma unroll 2
-                for (int i = 0; i < U::RPL; i++) {
-                    const int row = rg + U::RG * i;
-                    uint32_t w[U::W], lo[4], hi[4];
-                    load_words(raw + row * F::DC + U::BPL * c, w, U::W);
-                    codes_of<BITS>(w, lo, hi);
-                    if constexpr (kv) {
-                        const uint32_t vs = uint32_t(reinterpret_cast<const uint16_t*>(raw + 16 * F::DC)[row]) * 0x10001u;
-                        const uint32_t vb = uint32_t(reinterpret_cast<const uint16_t*>(raw + 16 * F::DC + 32)[row]) * 0x10001u;
+                codes_of<BITS>(w, lo, hi);
+                if constexpr (kv) {
+                    const uint32_t vs = uint32_t(reinterpret_cast<const uint16_t*>(u8 + 16 * F::DC)[row]) * 0x10001u;
+                    const uint32_t vb = uint32_t(reinterpret_cast<const uint16_t*>(u8 + 16 * F::DC + 32)[row]) * 0x10001u;
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            lo[j] = h2_fma_u(lo[j], vs, vb);
-                            hi[j] = h2_fma_u(hi[j], vs, vb);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            lo[j] = h2_fma_u(lo[j], s[j], b[j]);
-                            hi[j] = h2_fma_u(hi[j], s[4 + j], b[4 + j]);
-                        }
+                    for (int j = 0; j < 4; j++) {
+                        lo[j] = h2_fma_u(lo[j], vs, vb);
+                        hi[j] = h2_fma_u(hi[j], vs, vb);
                     }
-                    const uint32_t at_lo = dst + tile_off(16 * u + row, lo_c), at_hi = dst + tile_off(16 * u + row, hi_c);
-                    st_chunk(flip ? at_hi : at_lo, flip ? hi[0] : lo[0], flip ? hi[1] : lo[1], flip ? hi[2] : lo[2], flip ? hi[3] : lo[3]);
-                    st_chunk(flip ? at_lo : at_hi, flip ? lo[0] : hi[0], flip ? lo[1] : hi[1], flip ? lo[2] : hi[2], flip ? lo[3] : hi[3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        lo[j] = h2_fma_u(lo[j], s[j], b[j]);
+                        hi[j] = h2_fma_u(hi[j], s[4 + j], b[4 + j]);
+                    }
+                }
+                const uint32_t flip = U::RG == 4 && (i & 1) ? 64 : 0;              // rows 4 apart: the swizzle's bit 2
+                st_chunk(dst + ((at_a ^ flip) + U::RG * 128 * i), lo[0], lo[1], lo[2], lo[3]);
+                st_chunk(dst + ((at_b ^ flip) + U::RG * 128 * i), hi[0], hi[1], hi[2], hi[3]);
+            }
+        };
+        for (int x = wid - 8; x < M::NS; x += TC_NPROD) bring(x, block_of(x));
+        int x = wid - 8, slot = x;                                                 // slot = x % NS
+        if (x < units) {
+            const int j0 = first_token(x), kind = kind_of(j0);
+            if (kind != 1) {
+#pragma unroll
+                for (int i = 0; i < NI; i++) raw[i] = unpacked(x & 8, j0, kind, i);
+            }
+        }
+        uint32_t phase = 0;
+        for (; x < units && ok; x += TC_NPROD) {
+            const int n = x >> 4, st = n & 1, u = x & 7, j0 = first_token(x), kind = kind_of(j0);
+            const bool kv = x & 8;
+            const int32_t blk = block_of(x + M::NS);
+            const int xn = x + TC_NPROD, jn = xn < units ? first_token(xn) : 0, kindn = xn < units ? kind_of(jn) : 1;
+            const uint32_t dst = base + (kv ? M::V : M::K) + st * M::TILE + u * 2048;
+            const uint32_t bar_e = (kv ? v_empty : k_empty) + 8 * st, bar_f = (kv ? v_full : k_full) + 8 * st;
+            if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
+            if (kind == 1) {
+                if (ok && !(was_brought(x, slot) && wait(r_full + 8 * slot, phase))) ok = false;
+                if (kv) packed_unit(IC<1>{}, x, dst, slot);
+                else packed_unit(IC<0>{}, x, dst, slot);
+                if (kindn != 1) {
+#pragma unroll
+                    for (int i = 0; i < NI; i++) raw[i] = unpacked(xn & 8, jn, kindn, i);
                 }
             } else {
-                // new rows, the unfinished page, unseen tokens: 8-channel chunks of a row, CH lanes per row
-                constexpr int RPI = WARP / CH, NI = 16 / RPI;                      // rows per step, steps
-                const int cc = lane % CH, r0 = lane / CH;
-                uint4 raw[NI];
+                // convert a row, then fetch the same row of this warp's next unit
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
-                    const int j = j0 + i * RPI + r0;
-                    const bool see = kind == 2 || (kind == 3 && kt.seen(j, t.p1));
-                    raw[i] = make_uint4(0, 0, 0, 0);
-                    if (see && j >= t.ctx) {
-                        const IN* src = kv ? vn + int64_t(j - t.ctx) * a.v_stride : kn + int64_t(j - t.ctx) * a.k_stride;
-                        raw[i] = *reinterpret_cast<const uint4*>(src + 8 * cc);
-                    } else if (!kv && see && j >= full) {
-                        raw[i] = *reinterpret_cast<const uint4*>(tail + (j % P) * D + 8 * cc);
-                    }
-                }
-                float rf8[8];
-                if constexpr (!kv) {
-#pragma unroll
-                    for (int k = 0; k < 8; k++) rf8[k] = ref[8 * cc + k];
-                }
-                if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
-#pragma unroll
-                for (int i = 0; i < NI; i++) {
-                    const int row = 16 * u + i * RPI + r0, j = j0 + i * RPI + r0;
+                    const int row = i * RPI + r0, j = j0 + row;
                     const IN* e = reinterpret_cast<const IN*>(&raw[i]);
-                    const bool sub = kind == 2 || (kind == 3 && kt.seen(j, t.p1));
+                    const bool sub = !kv && (kind == 2 || (kind == 3 && kt.seen(j, t.p1)));
                     uint32_t p[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        p[k] = kv || !sub ? h2_pack(to_f32(e[2 * k]), to_f32(e[2 * k + 1]))
-                                          : h2_pack(to_f32(e[2 * k]) - rf8[2 * k], to_f32(e[2 * k + 1]) - rf8[2 * k + 1]);
+                        p[k] = h2_pack(to_f32(e[2 * k]) - (sub ? rf8[2 * k] : 0.0f), to_f32(e[2 * k + 1]) - (sub ? rf8[2 * k + 1] : 0.0f));
                     st_chunk(dst + tile_off(row, cc), p[0], p[1], p[2], p[3]);
+                    if (kindn != 1) raw[i] = unpacked(xn & 8, jn, kindn, i);
                 }
                 if (kind == 3) {                                                   // its cached tokens, one row after the other
 #pragma unroll 1
                     for (int i = 0; i < NI; i++) {
-                        const int row = 16 * u + i * RPI + r0, j = j0 + i * RPI + r0;
+                        const int row = i * RPI + r0, j = j0 + row;
                         if (!kt.seen(j, t.p1) || j >= (kv ? t.ctx : full)) continue;
                         const uint8_t* rec = hcache + int64_t(bt[j / P]) * a.block_stride;
                         const int at = j % P;
@@ -648,7 +673,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                             y[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + at * F::DC, d)), h_load(rec + F::OFF_VS, at),
                                              h_load(rec + F::OFF_VB, at))
                                       : fmaf(float(code_at<D, BITS>(rec + at * F::DC, d)), h_load(rec + F::OFF_KS, d),
-                                             h_load(rec + F::OFF_KB, d)) - ref[d];
+                                             h_load(rec + F::OFF_KB, d)) - rf8[k];
                         }
                         st_chunk(dst + tile_off(row, cc), h2_pack(y[0], y[1]), h2_pack(y[2], y[3]), h2_pack(y[4], y[5]),
                                  h2_pack(y[6], y[7]));
@@ -656,17 +681,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 }
             }
             fence_async();
-            __syncwarp();
-            if (lane == 0) bar_arrive(bar_f);
-        };
-        for (int x = wid - 8; x < M::NS; x += TC_NPROD) bring(x, block_of(x));
-        int x = wid - 8;
-        for (; x < units && ok; x += TC_NPROD) {
-            const int32_t blk = block_of(x + M::NS);
-            if (x & 8) fill(IC<1>{}, x);
-            else fill(IC<0>{}, x);
             ok = __all_sync(0xffffffffu, ok);
-            if (ok && was_brought(x)) bring(x + M::NS, blk);                       // (units of a slot are brought in order)
+            if (lane == 0) bar_arrive(bar_f);
+            if (ok && was_brought(x, slot)) bring(x + M::NS, blk);                 // (units of a slot are brought in order)
+            slot += TC_NPROD;
+            if (slot >= M::NS) {
+                slot -= M::NS;
+                phase ^= 1;
+            }
         }
         if (!ok) {
             // given up: a bounded wait for the copies that this warp has issued and that may still be in flight
@@ -678,64 +700,80 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             for (int y = wid - 8; y < M::NS; y += TC_NPROD) landed(y);
             for (int y = x - TC_NPROD; y >= max(0, x - TC_NPROD - M::NS); y -= TC_NPROD) landed(y + M::NS);
         }
-    } else if (lane == 0) {
+    } else {
         // ---------------------------------------------------------------- the products, in the order of (tile, slot)
         // S of a pair goes out before O of the pair before it when the slots differ, so that one slot's softmax runs under
-        // the other's products; a slot's own S has to wait for its O product, which reads P from S's columns.
+        // the other's products; a slot's own S has to wait for its O product, which reads P from S's columns.  The warp
+        // walks together on warp-uniform values (the products' operands live in uniform registers), one thread issues.
         constexpr uint32_t ID_S = instr_desc(128, TC_TN, false), ID_O = instr_desc(128, D, true);
+        auto uni = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+        const bool leader = elect_one();
+        const uint32_t tm = uni(tmem);
         const uint64_t q_desc = smem_desc(base + M::Q, 16, 1024), k_desc = smem_desc(base + M::K, 16, 1024);
         const uint64_t v_desc = smem_desc(base + M::V, M::BLK, 1024);
-        uint32_t done[2] = {0, 0};                                                 // O products issued per slot
-        int pit = -1, ps = 0;                                                      // the pair whose O product is due
-        int it = i0, slot = active(0, i0) ? 0 : 1;
-        while (ok && (it < i1 || pit >= 0)) {
-            const bool more = it < i1, s_first = pit < 0 || (more && slot != ps);
+        const int n1 = uni(i1 - i0), e0 = uni(end0 - i0), g0 = uni(gap0 - i0), g1 = uni(gap1 - i0), pr = uni(paired);
+        auto works = [&](int slot, int n) -> bool {                                // active() of tile i0 + n
+            return pr ? (slot == 0 ? n < e0 : n < g0 || n >= g1) : (n & 1) == slot;
+        };
+        uint32_t done0 = 0, done1 = 0;                                             // O products issued per slot
+        int pn = -1, ps = 0;                                                       // the pair whose O product is due
+        int n = 0, slot = works(0, 0) ? 0 : 1;
+        while (ok && (n < n1 || pn >= 0)) {
+            const bool more = n < n1, s_first = pn < 0 || (more && slot != ps);
 #pragma unroll 1
             for (int step = 0; step < 2 && ok; step++) {
                 if ((step == 0) == s_first) {
                     if (!more) continue;
-                    const int n = it - i0, st = n & 1;
-                    ok = wait(k_full + 8 * st, (n >> 1) & 1);
+                    const int st = n & 1;
+                    ok = __all_sync(0xffffffffu, wait(k_full + 8 * st, (n >> 1) & 1));
                     if (!ok) break;
                     fence_after();
-                    const uint64_t qd = q_desc + (paired && slot ? M::TILE >> 4 : 0), kd = k_desc + st * (M::TILE >> 4);
+                    if (leader) {
+                        const uint64_t qd = q_desc + (pr && slot ? M::TILE >> 4 : 0), kd = k_desc + st * (M::TILE >> 4);
 #pragma unroll
-                    for (int k = 0; k < D / 16; k++) {
-                        const uint32_t off = ((k >> 2) * M::BLK + (k & 3) * 32) >> 4;
-                        mma_ss(tmem + 128 * slot, qd + off, kd + off, ID_S, k > 0);
+                        for (int k = 0; k < D / 16; k++) {
+                            const uint32_t off = ((k >> 2) * M::BLK + (k & 3) * 32) >> 4;
+                            mma_ss(tm + 128 * slot, qd + off, kd + off, ID_S, k > 0);
+                        }
+                        mma_commit(s_full + 8 * slot);
+                        if (slot == 1 || !works(1, n)) mma_commit(k_empty + 8 * st);
                     }
-                    mma_commit(s_full + 8 * slot);
-                    if (slot == 1 || !active(1, it)) mma_commit(k_empty + 8 * st);
-                } else if (pit >= 0) {
-                    const int n = pit - i0, st = n & 1;
-                    ok = wait(v_full + 8 * st, (n >> 1) & 1) && wait(p_full + 8 * ps, (ps ? done[1] : done[0]) & 1);
+                    __syncwarp();
+                } else if (pn >= 0) {
+                    const int st = pn & 1;
+                    const uint32_t d = ps ? done1 : done0;
+                    ok = __all_sync(0xffffffffu, wait(v_full + 8 * st, (pn >> 1) & 1) && wait(p_full + 8 * ps, d & 1));
                     if (!ok) break;
                     fence_after();
-                    const uint64_t vd = v_desc + st * (M::TILE >> 4);
-                    const bool acc = (ps ? done[1] : done[0]) > 0;
+                    if (leader) {
+                        const uint64_t vd = v_desc + st * (M::TILE >> 4);
 #pragma unroll
-                    for (int k = 0; k < TC_TN / 16; k++)
-                        mma_ts(tmem + 256 + 128 * ps, tmem + 128 * ps + 8 * k, vd + k * (2048 >> 4), ID_O, acc || k > 0);
-                    if (ps) done[1]++;
-                    else done[0]++;
-                    if (ps == 1 || !active(1, pit)) mma_commit(v_empty + 8 * st);
+                        for (int k = 0; k < TC_TN / 16; k++)
+                            mma_ts(tm + 256 + 128 * ps, tm + 128 * ps + 8 * k, vd + k * (2048 >> 4), ID_O, d > 0 || k > 0);
+                        if (ps == 1 || !works(1, pn)) mma_commit(v_empty + 8 * st);
+                    }
+                    __syncwarp();
+                    if (ps) done1++;
+                    else done0++;
                 }
             }
-            pit = more ? it : -1;
+            pn = more ? n : -1;
             ps = slot;
             if (more) {                                                            // the next active pair
-                if (slot == 0 && active(1, it)) {
+                if (slot == 0 && works(1, n)) {
                     slot = 1;
                 } else {
-                    it++;
-                    slot = it < i1 && active(0, it) ? 0 : 1;
+                    n++;
+                    slot = works(0, n) ? 0 : 1;
                 }
             }
         }
         // both slots' outputs; nothing of this block is in flight when it ends, whatever ended the loop
-        mma_commit(o_full);
-        mma_commit(o_full + 8);
-        for (int i = 0; i < 1 << 20 && !(mbar_done(o_full, 0) && mbar_done(o_full + 8, 0)); i++) {
+        if (leader) {
+            mma_commit(o_full);
+            mma_commit(o_full + 8);
+            for (int i = 0; i < 1 << 20 && !(mbar_done(o_full, 0) && mbar_done(o_full + 8, 0)); i++) {
+            }
         }
     }
     __syncwarp();
