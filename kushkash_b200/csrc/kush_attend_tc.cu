@@ -32,10 +32,10 @@ struct TcSmem {
     static constexpr int DC = BITS == 8 ? D : D / 2;
     static constexpr int BLK = 128 * 128;                    // 128 rows x 64 channels of fp16: one swizzled block
     static constexpr int TILE = BLK * (D / 64);
-    // ring of packed units on their way in: 16 rows of codes, then the key scales and biases (values: 16 of each)
-    static constexpr int SLOT = 16 * DC + 4 * D, NS = D == 64 ? 24 : BITS == 4 ? 20 : 12;
+    // packed units on their way in, R slots for each producing warp: 16 rows of codes, then 16 value scales and biases
+    static constexpr int SLOT = 16 * DC + 64, R = D == 64 || BITS == 4 ? 4 : 2, NS = TC_NPROD * R;
     static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, RING = V + 2 * TILE, REF = RING + NS * SLOT;   // REF: fp32 [D]
-    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * (14 + NS), BROUGHT = MISC + 16, BYTES = BROUGHT + 4 * NS + 1024;   // + alignment
+    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * (14 + NS), BYTES = MISC + 16 + 1024;                // + alignment
     static_assert(BYTES <= 232448, "shared memory of a block");
 };
 
@@ -242,14 +242,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64,
                    p_full = bars + 80, o_full = bars + 96, r_full = bars + 112;    // pairs: [stage] or [slot]; [ring]
     volatile int* gave_up = reinterpret_cast<volatile int*>(sm + M::MISC);
-    volatile int* brought = reinterpret_cast<volatile int*>(sm + M::BROUGHT);    // [ring] the unit last brought to a slot
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + M::MISC + 4);
     if (tid == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(sm + M::BARS);
         const int count[7] = {8, 1, 8, 1, 1, 4, 1};
         for (int i = 0; i < 14 + M::NS; i++) mbar_init(b + i, i < 14 ? count[i / 2] : 1);
         *gave_up = 0;
-        for (int i = 0; i < M::NS; i++) brought[i] = -1;
         fence_mbar_init();
     }
     if (wid == 15) {
@@ -518,53 +516,55 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         float rf8[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) rf8[k] = ref[8 * cc + k];
-        // The stream of units x: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp converts every 7th.
-        // Packed units come through a ring of NS slots, in stream order; whoever has converted unit x brings x + NS into
-        // its slot (units that are not packed only complete the slot's phase).
-        const int units = 16 * (i1 - i0);
-        auto first_token = [&](int x) { return kt.tile(i0 + (x >> 4)) * TC_TN + 16 * (x & 7); };
-        auto kind_of = [&](int j0) {                                               // 0 unseen, 1 packed, 2 new rows, 3 mixed
-            if (j0 > t.p1 || (j0 + 15 < kt.lo && j0 >= kt.ns)) return 0;
-            return j0 + 16 <= full ? 1 : j0 >= t.ctx && j0 + 15 <= t.p1 ? 2 : 3;
-        };
-        auto block_of = [&](int x) -> int32_t {                                    // block id of a packed unit
-            if (x >= units) return 0;
-            const int j0 = first_token(x);
-            return kind_of(j0) == 1 ? bt[j0 / P] : 0;
-        };
-        auto bring = [&](int x, int32_t blk) {
-            if (x >= units || lane != 0) return;
-            const int slot = x % M::NS, j0 = first_token(x);
-            const uint32_t bar = r_full + 8 * slot, dst = base + M::RING + slot * M::SLOT;
-            // x - NS has landed and is converted.  The slot is marked after this phase's one arrival: who sees the mark may
-            // bring x + NS, whose arrival must find this phase closed.
-            if (kind_of(j0) != 1) {
-                bar_arrive(bar);
-                brought[slot] = x;
-                return;
+        // The stream of units x: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp's k-th is
+        // x = w + 7 k.  Where its units come from is worked out for 32 of them at a time, a lane each.
+        const int units = 16 * (i1 - i0), w = wid - 8, mine = w < units ? (units - w + TC_NPROD - 1) / TC_NPROD : 0;
+        const bool leader = elect_one();
+        int32_t from[2], blk[2];                                                   // of units 32 i + lane, two batches: first
+        auto batch = [&](int i, int32_t& f, int32_t& bl) {                         // token | kind, and the packed unit's block
+            const int k = 32 * i + lane, x = w + TC_NPROD * k;
+            f = bl = 0;
+            if (k < mine) {
+                const int j0 = kt.tile(i0 + (x >> 4)) * TC_TN + 16 * (x & 7);
+                // 0 no row sees a token of it, 1 packed, 2 new rows, 3 mixed
+                const int kind = j0 > t.p1 || (j0 + 15 < kt.lo && j0 >= kt.ns) ? 0 : j0 + 16 <= full ? 1
+                                 : j0 >= t.ctx && j0 + 15 <= t.p1 ? 2 : 3;
+                f = j0 | kind;
+                if (kind == 1) bl = bt[j0 / P];
             }
-            const uint8_t* rec = hcache + int64_t(blk) * a.block_stride;
-            const int r0 = j0 % P;
-            if (x & 8) {
-                bar_expect(bar, 16 * F::DC + 64);
-                brought[slot] = x;
-                bulk_in(dst, rec + F::OFF_VQ + r0 * F::DC, 16 * F::DC, bar);
-                if constexpr (P == 16) {
-                    bulk_in(dst + 16 * F::DC, rec + F::OFF_VS, 64, bar);           // scales, then biases
+        };
+        batch(0, from[0], blk[0]);
+        batch(1, from[1], blk[1]);
+        auto of = [&](const int32_t (&v)[2], int k, int now) {                     // of unit k, in batch now or now + 1
+            const int32_t v0 = __shfl_sync(0xffffffffu, v[0], k & 31), v1 = __shfl_sync(0xffffffffu, v[1], k & 31);
+            return (k >> 5) == now ? v0 : v1;
+        };
+        const uint32_t my_ring = base + M::RING + w * M::R * M::SLOT, my_bar = r_full + 8 * w * M::R;
+        uint32_t phases = 0, coming = 0;                                           // bit per slot: phase to wait for, copy under way
+        auto bring = [&](int k, int now) {                                         // unit k into its slot k % R, if it is packed
+            const int32_t f = of(from, k, now), bl = of(blk, k, now);
+            if (k >= mine || (f & 15) != 1) return;
+            const int slot = k % M::R, r0 = (f & ~15) % P;
+            coming |= 1u << slot;
+            if (leader) {
+                const uint32_t bar = my_bar + 8 * slot, dst = my_ring + slot * M::SLOT;
+                const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
+                if ((w + TC_NPROD * k) & 8) {
+                    bar_expect(bar, 16 * F::DC + 64);
+                    bulk_in(dst, rec + F::OFF_VQ + r0 * F::DC, 16 * F::DC, bar);
+                    if constexpr (P == 16) {
+                        bulk_in(dst + 16 * F::DC, rec + F::OFF_VS, 64, bar);       // scales, then biases
+                    } else {
+                        bulk_in(dst + 16 * F::DC, rec + F::OFF_VS + 2 * r0, 32, bar);
+                        bulk_in(dst + 16 * F::DC + 32, rec + F::OFF_VB + 2 * r0, 32, bar);
+                    }
                 } else {
-                    bulk_in(dst + 16 * F::DC, rec + F::OFF_VS + 2 * r0, 32, bar);
-                    bulk_in(dst + 16 * F::DC + 32, rec + F::OFF_VB + 2 * r0, 32, bar);
+                    bar_expect(bar, 16 * F::DC);
+                    bulk_in(dst, rec + r0 * F::DC, 16 * F::DC, bar);
                 }
-            } else {
-                bar_expect(bar, 16 * F::DC + 4 * D);
-                brought[slot] = x;
-                bulk_in(dst, rec + r0 * F::DC, 16 * F::DC, bar);
-                bulk_in(dst + 16 * F::DC, rec + F::OFF_KS, 4 * D, bar);
             }
+            __syncwarp();
         };
-        // A warp may be ahead of the one that converts x - NS and then brings x: a parity alone does not tell x's phase from
-        // the one two before it, so the slot says first which unit was brought.
-        auto was_brought = [&](int x, int slot) -> bool { return until([&] { return brought[slot] == x; }); };
         // a row of an unpacked unit (new rows, the unfinished page, unseen tokens): 16 bytes of row i * RPI + r0
         auto unpacked = [&](bool kv, int j0, int kind, int i) -> uint4 {
             const int j = j0 + i * RPI + r0;
@@ -575,19 +575,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 src = tail + (j % P) * D;
             return src ? *reinterpret_cast<const uint4*>(src + 8 * cc) : make_uint4(0, 0, 0, 0);
         };
-        uint4 raw[NI];                                                             // this warp's next unpacked unit
-        auto packed_unit = [&](auto kvc, int x, uint32_t dst, int slot) {
+        // what is fetched into registers for this warp's next unit: an unpacked unit's rows, or a packed key unit's scales
+        // and biases (first two words of four: chunk a's, b's scales, then biases)
+        uint4 raw[NI < 4 ? 4 : NI];
+        auto fetch_scales = [&](int32_t bl) {
+            const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
+            raw[0] = *reinterpret_cast<const uint4*>(rec + F::OFF_KS + 16 * c_a);
+            raw[1] = *reinterpret_cast<const uint4*>(rec + F::OFF_KS + 16 * c_b);
+            raw[2] = *reinterpret_cast<const uint4*>(rec + F::OFF_KB + 16 * c_a);
+            raw[3] = *reinterpret_cast<const uint4*>(rec + F::OFF_KB + 16 * c_b);
+        };
+        auto packed_unit = [&](auto kvc, const uint8_t* u8, uint32_t dst, const uint32_t (&s)[8], const uint32_t (&b)[8]) {
             constexpr bool kv = decltype(kvc)::value;                              // values (else keys)
-            const uint8_t* u8 = sm + M::RING + slot * M::SLOT;
-            uint32_t s[8], b[8];
-            if constexpr (!kv) {
-                load_words(u8 + 16 * F::DC + 16 * c_a, s, 4);
-                load_words(u8 + 16 * F::DC + 16 * c_b, s + 4, 4);
-                load_words(u8 + 16 * F::DC + 2 * D + 16 * c_a, b, 4);
-                load_words(u8 + 16 * F::DC + 2 * D + 16 * c_b, b + 4, 4);
-#pragma unroll
-                for (int i = 0; i < 8; i++) b[i] = h2_sub_u(b[i], rf[i]);
-            }
 #pragma unroll
             for (int i = 0; i < U::RPL; i++) {
                 const int row = rg + U::RG * i;
@@ -619,34 +618,51 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 st_chunk(dst + ((at_b ^ flip) + U::RG * 128 * i), hi[0], hi[1], hi[2], hi[3]);
             }
         };
-        for (int x = wid - 8; x < M::NS; x += TC_NPROD) bring(x, block_of(x));
-        int x = wid - 8, slot = x;                                                 // slot = x % NS
-        if (x < units) {
-            const int j0 = first_token(x), kind = kind_of(j0);
-            if (kind != 1) {
+        for (int k = 0; k < M::R; k++) bring(k, 0);
+        auto fetch = [&](int k, int now) -> int32_t {                              // ahead of unit k; returns its first token | kind
+            const int32_t f = of(from, k, now), bl = of(blk, k, now);
+            if (k >= mine) return 1;
+            const int x = w + TC_NPROD * k;
+            if ((f & 15) != 1) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) raw[i] = unpacked(x & 8, j0, kind, i);
+                for (int i = 0; i < NI; i++) raw[i] = unpacked(x & 8, f & ~15, f & 15, i);
+            } else if (!(x & 8)) {
+                fetch_scales(bl);
             }
-        }
-        uint32_t phase = 0;
-        for (; x < units && ok; x += TC_NPROD) {
-            const int n = x >> 4, st = n & 1, u = x & 7, j0 = first_token(x), kind = kind_of(j0);
+            return f;
+        };
+        int32_t f = fetch(0, 0);
+        for (int k = 0, now = 0; k < mine && ok; k++) {
+            const int x = w + TC_NPROD * k, n = x >> 4, st = n & 1, u = x & 7, j0 = f & ~15, kind = f & 15;
             const bool kv = x & 8;
-            const int32_t blk = block_of(x + M::NS);
-            const int xn = x + TC_NPROD, jn = xn < units ? first_token(xn) : 0, kindn = xn < units ? kind_of(jn) : 1;
             const uint32_t dst = base + (kv ? M::V : M::K) + st * M::TILE + u * 2048;
             const uint32_t bar_e = (kv ? v_empty : k_empty) + 8 * st, bar_f = (kv ? v_full : k_full) + 8 * st;
-            if (n >= 2 && !wait(bar_e, ((n >> 1) - 1) & 1)) ok = false;
+            ok = wait(bar_e, ((n >> 1) - 1) & 1);                                  // (a fresh barrier lets tiles 0 and 1 pass)
             if (kind == 1) {
-                if (ok && !(was_brought(x, slot) && wait(r_full + 8 * slot, phase))) ok = false;
-                if (kv) packed_unit(IC<1>{}, x, dst, slot);
-                else packed_unit(IC<0>{}, x, dst, slot);
-                if (kindn != 1) {
+                const int slot = k % M::R;
+                const uint8_t* u8 = sm + M::RING + (w * M::R + slot) * M::SLOT;
+                uint32_t s[8], b[8];
+                if (!kv) {
+                    const uint32_t* r = reinterpret_cast<const uint32_t*>(raw);
 #pragma unroll
-                    for (int i = 0; i < NI; i++) raw[i] = unpacked(xn & 8, jn, kindn, i);
+                    for (int i = 0; i < 8; i++) {
+                        s[i] = r[i];
+                        b[i] = h2_sub_u(r[8 + i], rf[i]);
+                    }
                 }
+                f = fetch(k + 1, now);
+                if (ok) ok = wait(my_bar + 8 * slot, (phases >> slot) & 1);
+                if (ok) {
+                    phases ^= 1u << slot;
+                    coming &= ~(1u << slot);
+                }
+                if (kv) packed_unit(IC<1>{}, u8, dst, s, b);
+                else packed_unit(IC<0>{}, u8, dst, s, b);
             } else {
-                // convert a row, then fetch the same row of this warp's next unit
+                // convert a row, then fetch the same row of this warp's next unit if that is unpacked too
+                const int32_t fn = of(from, k + 1, now);
+                const int xn = x + TC_NPROD, jn = fn & ~15, kindn = fn & 15;
+                const bool again = k + 1 < mine && kindn != 1;
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
                     const int row = i * RPI + r0, j = j0 + row;
@@ -657,8 +673,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     for (int k = 0; k < 4; k++)
                         p[k] = h2_pack(to_f32(e[2 * k]) - (sub ? rf8[2 * k] : 0.0f), to_f32(e[2 * k + 1]) - (sub ? rf8[2 * k + 1] : 0.0f));
                     st_chunk(dst + tile_off(row, cc), p[0], p[1], p[2], p[3]);
-                    if (kindn != 1) raw[i] = unpacked(xn & 8, jn, kindn, i);
+                    if (again) raw[i] = unpacked(xn & 8, jn, kindn, i);
                 }
+                f = again ? fn : fetch(k + 1, now);
                 if (kind == 3) {                                                   // its cached tokens, one row after the other
 #pragma unroll 1
                     for (int i = 0; i < NI; i++) {
@@ -683,23 +700,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             fence_async();
             ok = __all_sync(0xffffffffu, ok);
             if (lane == 0) bar_arrive(bar_f);
-            if (ok && was_brought(x, slot)) bring(x + M::NS, blk);                 // (units of a slot are brought in order)
-            slot += TC_NPROD;
-            if (slot >= M::NS) {
-                slot -= M::NS;
-                phase ^= 1;
+            bring(k + M::R, now);
+            if ((k & 31) == 31) {
+                now++;
+                from[0] = from[1];
+                blk[0] = blk[1];
+                batch(now + 1, from[1], blk[1]);
             }
         }
-        if (!ok) {
-            // given up: a bounded wait for the copies that this warp has issued and that may still be in flight
-            auto landed = [&](int y) {
-                if (y >= units || kind_of(first_token(y)) != 1) return;
-                for (int i = 0; i < 1 << 16 && !mbar_done(r_full + 8 * (y % M::NS), (y / M::NS) & 1); i++) {
+        // given up: a bounded wait for this warp's copies that may still be in flight
+        for (int slot = 0; slot < M::R; slot++)
+            if (coming >> slot & 1)
+                for (int i = 0; i < 1 << 16 && !mbar_done(my_bar + 8 * slot, (phases >> slot) & 1); i++) {
                 }
-            };
-            for (int y = wid - 8; y < M::NS; y += TC_NPROD) landed(y);
-            for (int y = x - TC_NPROD; y >= max(0, x - TC_NPROD - M::NS); y -= TC_NPROD) landed(y + M::NS);
-        }
     } else {
         // ---------------------------------------------------------------- the products, in the order of (tile, slot)
         // S of a pair goes out before O of the pair before it when the slots differ, so that one slot's softmax runs under
