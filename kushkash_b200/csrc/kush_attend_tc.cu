@@ -27,15 +27,12 @@ constexpr float TC_TAU = 8.0f;
 
 __device__ int g_attend_error = 0;
 
-template <int D, int BITS>
+template <int D>
 struct TcSmem {
-    static constexpr int DC = BITS == 8 ? D : D / 2;
     static constexpr int BLK = 128 * 128;                    // 128 rows x 64 channels of fp16: one swizzled block
     static constexpr int TILE = BLK * (D / 64);
-    // packed units on their way in, R slots for each producing warp: 16 rows of codes, then 16 value scales and biases
-    static constexpr int SLOT = 16 * DC + 64, R = D == 64 || BITS == 4 ? 4 : 2, NS = TC_NPROD * R;
-    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, RING = V + 2 * TILE, REF = RING + NS * SLOT;   // REF: fp32 [D]
-    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * (14 + NS), BYTES = MISC + 16 + 1024;                // + alignment
+    static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, REF = V + 2 * TILE;               // REF: fp32 [D]
+    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * 14, BYTES = MISC + 16 + 1024;          // + alignment
     static_assert(BYTES <= 232448, "shared memory of a block");
 };
 
@@ -179,14 +176,9 @@ struct Unit {
     static constexpr int W = BITS / 2, BPL = 4 * W, LPR = F::DC / BPL, RG = WARP / LPR, RPL = 16 / RG;
 };
 
-// one thread: an untiled bulk copy into shared memory, completing on `bar` (16-byte addresses and size; no multicast)
-__device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+// a packed unit's bytes into L2, ahead of their loads (16-byte address and size)
+__device__ __forceinline__ void bulk_to_l2(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -213,7 +205,7 @@ template <int D, int BITS, int P, class IN>
 __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) {
     using F = Fmt<D, BITS, P>;
     using U = Unit<D, BITS, P>;
-    using M = TcSmem<D, BITS>;
+    using M = TcSmem<D>;
     constexpr int CH = D / 8;                                      // 8-channel chunks of a row
     extern __shared__ uint8_t smem_raw[];
     pdl_wait();
@@ -240,13 +232,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     float* ref = reinterpret_cast<float*>(sm + M::REF);
     const uint32_t bars = base + M::BARS;
     const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64,
-                   p_full = bars + 80, o_full = bars + 96, r_full = bars + 112;    // pairs: [stage] or [slot]; [ring]
+                   p_full = bars + 80, o_full = bars + 96;                         // pairs: [stage] or [slot]
     volatile int* gave_up = reinterpret_cast<volatile int*>(sm + M::MISC);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + M::MISC + 4);
     if (tid == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(sm + M::BARS);
         const int count[7] = {8, 1, 8, 1, 1, 4, 1};
-        for (int i = 0; i < 14 + M::NS; i++) mbar_init(b + i, i < 14 ? count[i / 2] : 1);
+        for (int i = 0; i < 14; i++) mbar_init(b + i, count[i / 2]);
         *gave_up = 0;
         fence_mbar_init();
     }
@@ -517,10 +509,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
 #pragma unroll
         for (int k = 0; k < 8; k++) rf8[k] = ref[8 * cc + k];
         // The stream of units x: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp's k-th is
-        // x = w + 7 k.  Where its units come from is worked out for 32 of them at a time, a lane each.
+        // x = w + 7 k.  Where its units come from is worked out for 32 of them at a time, a lane each, which also asks for
+        // their bytes into L2: a unit is then loaded into registers while the one before it is converted.
         const int units = 16 * (i1 - i0), w = wid - 8, mine = w < units ? (units - w + TC_NPROD - 1) / TC_NPROD : 0;
-        const bool leader = elect_one();
-        int32_t from[2], blk[2];                                                   // of units 32 i + lane, two batches: first
         auto batch = [&](int i, int32_t& f, int32_t& bl) {                         // token | kind, and the packed unit's block
             const int k = 32 * i + lane, x = w + TC_NPROD * k;
             f = bl = 0;
@@ -530,41 +521,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 const int kind = j0 > t.p1 || (j0 + 15 < kt.lo && j0 >= kt.ns) ? 0 : j0 + 16 <= full ? 1
                                  : j0 >= t.ctx && j0 + 15 <= t.p1 ? 2 : 3;
                 f = j0 | kind;
-                if (kind == 1) bl = bt[j0 / P];
-            }
-        };
-        batch(0, from[0], blk[0]);
-        batch(1, from[1], blk[1]);
-        auto of = [&](const int32_t (&v)[2], int k, int now) {                     // of unit k, in batch now or now + 1
-            const int32_t v0 = __shfl_sync(0xffffffffu, v[0], k & 31), v1 = __shfl_sync(0xffffffffu, v[1], k & 31);
-            return (k >> 5) == now ? v0 : v1;
-        };
-        const uint32_t my_ring = base + M::RING + w * M::R * M::SLOT, my_bar = r_full + 8 * w * M::R;
-        uint32_t phases = 0, coming = 0;                                           // bit per slot: phase to wait for, copy under way
-        auto bring = [&](int k, int now) {                                         // unit k into its slot k % R, if it is packed
-            const int32_t f = of(from, k, now), bl = of(blk, k, now);
-            if (k >= mine || (f & 15) != 1) return;
-            const int slot = k % M::R, r0 = (f & ~15) % P;
-            coming |= 1u << slot;
-            if (leader) {
-                const uint32_t bar = my_bar + 8 * slot, dst = my_ring + slot * M::SLOT;
-                const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
-                if ((w + TC_NPROD * k) & 8) {
-                    bar_expect(bar, 16 * F::DC + 64);
-                    bulk_in(dst, rec + F::OFF_VQ + r0 * F::DC, 16 * F::DC, bar);
-                    if constexpr (P == 16) {
-                        bulk_in(dst + 16 * F::DC, rec + F::OFF_VS, 64, bar);       // scales, then biases
-                    } else {
-                        bulk_in(dst + 16 * F::DC, rec + F::OFF_VS + 2 * r0, 32, bar);
-                        bulk_in(dst + 16 * F::DC + 32, rec + F::OFF_VB + 2 * r0, 32, bar);
-                    }
-                } else {
-                    bar_expect(bar, 16 * F::DC);
-                    bulk_in(dst, rec + r0 * F::DC, 16 * F::DC, bar);
+                if (kind == 1) {
+                    bl = bt[j0 / P];
+                    const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
+                    bulk_to_l2(rec + (x & 8 ? F::OFF_VQ : 0) + j0 % P * F::DC, 16 * F::DC);
+                    if (j0 % P == 0 && !(x & 8)) bulk_to_l2(rec + F::OFF_KS, F::RB - F::OFF_KS);
                 }
             }
-            __syncwarp();
         };
+        int32_t from, blk, from1, blk1;                                            // of units 32 i + lane; of the next batch
+        batch(0, from, blk);
+        batch(1, from1, blk1);
         // a row of an unpacked unit (new rows, the unfinished page, unseen tokens): 16 bytes of row i * RPI + r0
         auto unpacked = [&](bool kv, int j0, int kind, int i) -> uint4 {
             const int j = j0 + i * RPI + r0;
@@ -575,94 +542,105 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 src = tail + (j % P) * D;
             return src ? *reinterpret_cast<const uint4*>(src + 8 * cc) : make_uint4(0, 0, 0, 0);
         };
-        // what is fetched into registers for this warp's next unit: an unpacked unit's rows, or a packed key unit's scales
-        // and biases (first two words of four: chunk a's, b's scales, then biases)
-        uint4 raw[NI < 4 ? 4 : NI];
-        auto fetch_scales = [&](int32_t bl) {
-            const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
-            raw[0] = *reinterpret_cast<const uint4*>(rec + F::OFF_KS + 16 * c_a);
-            raw[1] = *reinterpret_cast<const uint4*>(rec + F::OFF_KS + 16 * c_b);
-            raw[2] = *reinterpret_cast<const uint4*>(rec + F::OFF_KB + 16 * c_a);
-            raw[3] = *reinterpret_cast<const uint4*>(rec + F::OFF_KB + 16 * c_b);
-        };
-        auto packed_unit = [&](auto kvc, const uint8_t* u8, uint32_t dst, const uint32_t (&s)[8], const uint32_t (&b)[8]) {
-            constexpr bool kv = decltype(kvc)::value;                              // values (else keys)
-#pragma unroll
-            for (int i = 0; i < U::RPL; i++) {
-                const int row = rg + U::RG * i;
-                uint32_t w[U::W], lo[4], hi[4];
-                if constexpr (BITS == 4) {
-                    load_words(u8 + row * F::DC + 8 * c, w, 2);
-                } else {
-                    load_words(u8 + row * F::DC + 8 * c_a, w, 2);
-                    load_words(u8 + row * F::DC + 8 * c_b, w + 2, 2);
-                }
-                codes_of<BITS>(w, lo, hi);
-                if constexpr (kv) {
-                    const uint32_t vs = uint32_t(reinterpret_cast<const uint16_t*>(u8 + 16 * F::DC)[row]) * 0x10001u;
-                    const uint32_t vb = uint32_t(reinterpret_cast<const uint16_t*>(u8 + 16 * F::DC + 32)[row]) * 0x10001u;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        lo[j] = h2_fma_u(lo[j], vs, vb);
-                        hi[j] = h2_fma_u(hi[j], vs, vb);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        lo[j] = h2_fma_u(lo[j], s[j], b[j]);
-                        hi[j] = h2_fma_u(hi[j], s[4 + j], b[4 + j]);
-                    }
-                }
-                const uint32_t flip = U::RG == 4 && (i & 1) ? 64 : 0;              // rows 4 apart: the swizzle's bit 2
-                st_chunk(dst + ((at_a ^ flip) + U::RG * 128 * i), lo[0], lo[1], lo[2], lo[3]);
-                st_chunk(dst + ((at_b ^ flip) + U::RG * 128 * i), hi[0], hi[1], hi[2], hi[3]);
-            }
-        };
-        for (int k = 0; k < M::R; k++) bring(k, 0);
-        auto fetch = [&](int k, int now) -> int32_t {                              // ahead of unit k; returns its first token | kind
-            const int32_t f = of(from, k, now), bl = of(blk, k, now);
+        // What is fetched into registers for this warp's next unit: an unpacked unit's rows; a packed one's codes (words
+        // [0, RPL W)) and, for keys, its scales and biases of chunks a and b (words [16, 32)), for values the scale of row
+        // lane or the bias of row lane - 16 (word 16).
+        constexpr int NRAW = NI < 8 ? 8 : NI;
+        uint4 raw[NRAW];
+        uint32_t* const rw = reinterpret_cast<uint32_t*>(raw);
+        auto fetch = [&](int k) -> int32_t {                                       // returns its first token | kind
             if (k >= mine) return 1;
-            const int x = w + TC_NPROD * k;
+            if ((k & 31) == 0 && k > 0) {
+                from = from1;
+                blk = blk1;
+                batch(k / 32 + 1, from1, blk1);
+            }
+            const int32_t f = __shfl_sync(0xffffffffu, from, k & 31), bl = __shfl_sync(0xffffffffu, blk, k & 31);
+            const int x = w + TC_NPROD * k, j0 = f & ~15;
+            const bool kv = x & 8;
             if ((f & 15) != 1) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) raw[i] = unpacked(x & 8, f & ~15, f & 15, i);
-            } else if (!(x & 8)) {
-                fetch_scales(bl);
+                for (int i = 0; i < NI; i++) raw[i] = unpacked(kv, j0, f & 15, i);
+                return f;
+            }
+            const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
+            const uint8_t* rows = rec + (kv ? F::OFF_VQ : 0) + (j0 % P + rg) * F::DC;
+#pragma unroll
+            for (int i = 0; i < U::RPL; i++) {
+                if constexpr (BITS == 4) {
+                    load_words(rows + U::RG * i * F::DC + 8 * c, rw + 2 * i, 2);
+                } else if constexpr (D == 128) {                                   // the two halves in the order of the stores
+                    load_words(rows + U::RG * i * F::DC + 8 * c_a, rw + 4 * i, 2);
+                    load_words(rows + U::RG * i * F::DC + 8 * c_b, rw + 4 * i + 2, 2);
+                } else {
+                    load_words(rows + U::RG * i * F::DC + 16 * c, rw + 4 * i, 4);
+                }
+            }
+            if (kv) {
+                rw[16] = reinterpret_cast<const uint16_t*>(rec + (lane < 16 ? F::OFF_VS : F::OFF_VB))[j0 % P + (lane & 15)];
+            } else {
+                raw[4] = *reinterpret_cast<const uint4*>(rec + F::OFF_KS + 16 * c_a);
+                raw[5] = *reinterpret_cast<const uint4*>(rec + F::OFF_KS + 16 * c_b);
+                raw[6] = *reinterpret_cast<const uint4*>(rec + F::OFF_KB + 16 * c_a);
+                raw[7] = *reinterpret_cast<const uint4*>(rec + F::OFF_KB + 16 * c_b);
             }
             return f;
         };
-        int32_t f = fetch(0, 0);
-        for (int k = 0, now = 0; k < mine && ok; k++) {
+        auto store_row = [&](uint32_t dst, int i, const uint32_t (&lo)[4], const uint32_t (&hi)[4]) {
+            const uint32_t flip = U::RG == 4 && (i & 1) ? 64 : 0;                  // rows 4 apart: the swizzle's bit 2
+            st_chunk(dst + ((at_a ^ flip) + U::RG * 128 * i), lo[0], lo[1], lo[2], lo[3]);
+            st_chunk(dst + ((at_b ^ flip) + U::RG * 128 * i), hi[0], hi[1], hi[2], hi[3]);
+        };
+        int32_t f = fetch(0);
+        for (int k = 0; k < mine && ok; k++) {
             const int x = w + TC_NPROD * k, n = x >> 4, st = n & 1, u = x & 7, j0 = f & ~15, kind = f & 15;
             const bool kv = x & 8;
             const uint32_t dst = base + (kv ? M::V : M::K) + st * M::TILE + u * 2048;
             const uint32_t bar_e = (kv ? v_empty : k_empty) + 8 * st, bar_f = (kv ? v_full : k_full) + 8 * st;
-            ok = wait(bar_e, ((n >> 1) - 1) & 1);                                  // (a fresh barrier lets tiles 0 and 1 pass)
             if (kind == 1) {
-                const int slot = k % M::R;
-                const uint8_t* u8 = sm + M::RING + (w * M::R + slot) * M::SLOT;
-                uint32_t s[8], b[8];
-                if (!kv) {
-                    const uint32_t* r = reinterpret_cast<const uint32_t*>(raw);
+                uint32_t cw[U::RPL][U::W], sb[16];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        s[i] = r[i];
-                        b[i] = h2_sub_u(r[8 + i], rf[i]);
+                for (int i = 0; i < U::RPL * U::W; i++) cw[i / U::W][i % U::W] = rw[i];
+#pragma unroll
+                for (int i = 0; i < 16; i++) sb[i] = rw[16 + i];
+                f = fetch(k + 1);
+                ok = wait(bar_e, ((n >> 1) - 1) & 1);                              // (a fresh barrier lets tiles 0 and 1 pass)
+                if (kv) {
+#pragma unroll
+                    for (int i = 0; i < U::RPL; i++) {
+                        uint32_t lo[4], hi[4];
+                        codes_of<BITS>(cw[i], lo, hi);
+                        const int row = rg + U::RG * i;
+                        const uint32_t vs = __shfl_sync(0xffffffffu, sb[0], row) * 0x10001u;
+                        const uint32_t vb = __shfl_sync(0xffffffffu, sb[0], 16 + row) * 0x10001u;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            lo[j] = h2_fma_u(lo[j], vs, vb);
+                            hi[j] = h2_fma_u(hi[j], vs, vb);
+                        }
+                        store_row(dst, i, lo, hi);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sb[8 + i] = h2_sub_u(sb[8 + i], rf[i]);
+#pragma unroll
+                    for (int i = 0; i < U::RPL; i++) {
+                        uint32_t lo[4], hi[4];
+                        codes_of<BITS>(cw[i], lo, hi);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            lo[j] = h2_fma_u(lo[j], sb[j], sb[8 + j]);
+                            hi[j] = h2_fma_u(hi[j], sb[4 + j], sb[12 + j]);
+                        }
+                        store_row(dst, i, lo, hi);
                     }
                 }
-                f = fetch(k + 1, now);
-                if (ok) ok = wait(my_bar + 8 * slot, (phases >> slot) & 1);
-                if (ok) {
-                    phases ^= 1u << slot;
-                    coming &= ~(1u << slot);
-                }
-                if (kv) packed_unit(IC<1>{}, u8, dst, s, b);
-                else packed_unit(IC<0>{}, u8, dst, s, b);
             } else {
-                // convert a row, then fetch the same row of this warp's next unit if that is unpacked too
-                const int32_t fn = of(from, k + 1, now);
+                // convert a row, then fetch the same row of this warp's next unit if that is unpacked too (a new batch waits)
+                ok = wait(bar_e, ((n >> 1) - 1) & 1);
+                const int32_t fn = __shfl_sync(0xffffffffu, from, (k + 1) & 31);
                 const int xn = x + TC_NPROD, jn = fn & ~15, kindn = fn & 15;
-                const bool again = k + 1 < mine && kindn != 1;
+                const bool again = k + 1 < mine && kindn != 1 && ((k + 1) & 31) != 0;
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
                     const int row = i * RPI + r0, j = j0 + row;
@@ -675,7 +653,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     st_chunk(dst + tile_off(row, cc), p[0], p[1], p[2], p[3]);
                     if (again) raw[i] = unpacked(xn & 8, jn, kindn, i);
                 }
-                f = again ? fn : fetch(k + 1, now);
+                f = again ? fn : fetch(k + 1);
                 if (kind == 3) {                                                   // its cached tokens, one row after the other
 #pragma unroll 1
                     for (int i = 0; i < NI; i++) {
@@ -700,19 +678,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             fence_async();
             ok = __all_sync(0xffffffffu, ok);
             if (lane == 0) bar_arrive(bar_f);
-            bring(k + M::R, now);
-            if ((k & 31) == 31) {
-                now++;
-                from[0] = from[1];
-                blk[0] = blk[1];
-                batch(now + 1, from[1], blk[1]);
-            }
         }
-        // given up: a bounded wait for this warp's copies that may still be in flight
-        for (int slot = 0; slot < M::R; slot++)
-            if (coming >> slot & 1)
-                for (int i = 0; i < 1 << 16 && !mbar_done(my_bar + 8 * slot, (phases >> slot) & 1); i++) {
-                }
     } else {
         // ---------------------------------------------------------------- the products, in the order of (tile, slot)
         // S of a pair goes out before O of the pair before it when the slots differ, so that one slot's softmax runs under
@@ -819,7 +785,7 @@ int launch_attend_tc(int D, int bits, int P, int dtype, const AttendArgs& a, int
             return KUSH_ERR_UNSUPPORTED;
         } else {
             auto kern = attend_tc_kernel<Dc.value, Bc.value, Pc.value, IN>;
-            constexpr int smem = TcSmem<Dc.value, Bc.value>::BYTES;
+            constexpr int smem = TcSmem<Dc.value>::BYTES;
             const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
             if (e != cudaSuccess) return set_error(KUSH_ERR_CUDA, "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
             launch_pdl(kern, dim3(unsigned(tiles), a.H, a.n_splits), dim3(TC_THREADS), size_t(smem), stream, a);
