@@ -61,7 +61,15 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// the loads before it have arrived: `r`'s registers are defined from here on
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
@@ -322,7 +330,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         const float sc = fmaxf(fabsf(a.sm_log2), 1e-30f);                          // (a masked score stays -inf under scale 0)
         const uint32_t lanes = uint32_t(wrow) << 16;
         const uint32_t s_at = tmem + lanes + 128 * slot, o_at = tmem + lanes + 256 + 128 * slot;
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY;                                                       // the maximum in use, log2 units
+        float2 la = make_float2(0.0f, 0.0f), lb = la;                              // the weights' sum, in four parts
         int n = 0;                                                                 // tiles done by this slot
         for (int it = i0; it < i1; it++) {
             if (!active(slot, it)) continue;
@@ -340,7 +349,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     for (int c = 0; c < 4; c++) {
                         uint32_t x[32];
                         tmem_ld32(s_at + 32 * c, x);
-                        wait_ld();
+                        wait_ld(x);
                         const int h0 = hi - 32 * c, l0 = lo - 32 * c, k0 = sk - 32 * c;
 #pragma unroll
                         for (int i = 0; i < 32; i++)
@@ -349,45 +358,52 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     }
                     wait_st();
                 }
-                float mx = -INFINITY;
+                // One pass: 32 columns at a time, the next ones on their way from TMEM; the maximum in use moves when a piece
+                // passes it by 2^TAU (seldom after a row's first tile), and then takes O, the sum and this tile's earlier
+                // weights along.
+                auto move_max = [&](int c, float mx) {
+                    const bool up = mx > m + TC_TAU;
+                    const float corr = up ? ex2(m - mx) : 1.0f;                    // first scores: 2^-inf = 0
+                    if (up) m = mx;
+                    la = __fmul2_rn(la, make_float2(corr, corr));
+                    lb = __fmul2_rn(lb, make_float2(corr, corr));
+                    const __half2 ch = __float2half2_rn(corr);
 #pragma unroll 1
-                for (int c = 0; c < 4; c += 2) {
-                    uint32_t x[32], y[32];
-                    tmem_ld32(s_at + 32 * c, x);
-                    tmem_ld32(s_at + 32 * c + 32, y);
-                    wait_ld();
-                    float m4[4] = {mx, mx, mx, mx};
+                    for (int e = 0; e < (n > 0 ? D / 32 : 0); e++) {               // O (the slot's last product is done)
+                        uint32_t x[32];
+                        tmem_ld32(o_at + 32 * e, x);
+                        wait_ld(x);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) m4[i & 3] = max3(m4[i & 3], __uint_as_float(x[i]), __uint_as_float(y[i]));
-                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                }
-                mx *= sc;
-                const bool bump = mx > m + TC_TAU;                                 // (m = -inf: any score)
-                if (__any_sync(0xffffffffu, bump)) {
-                    const float mn = bump ? mx : m;
-                    const float corr = bump ? ex2(m - mn) : 1.0f;                  // first scores: 2^-inf = 0
-                    m = mn;
-                    l *= corr;
-                    if (n > 0) {                                                   // the slot's last product is done
-#pragma unroll 1
-                        for (int c = 0; c < D / 32; c++) {
-                            uint32_t x[32];
-                            tmem_ld32(o_at + 32 * c, x);
-                            wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
-                            tmem_st32(o_at + 32 * c, x);
-                        }
+                        for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
+                        tmem_st32(o_at + 32 * e, x);
                     }
-                }
-                const float mm = m == -INFINITY ? 0.0f : m;                        // nothing seen yet: weights 0
-                const float2 sc2 = make_float2(sc, sc), mm2 = make_float2(-mm, -mm);
-                float2 la = make_float2(0.0f, 0.0f), lb = la;
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    uint32_t x[32], p[16];
-                    tmem_ld32(s_at + 32 * c, x);
-                    wait_ld();
+                    for (int e = 0; e < c; e++) {                                  // P's pieces before this one
+                        uint32_t x[32], p[16];
+                        tmem_ld32(s_at + 16 * e, x);
+                        wait_ld(x);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&x[i]), ch);
+                            p[i] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        tmem_st16(s_at + 16 * e, p);
+                        wait_st();
+                    }
+                };
+                auto piece = [&](int c, const uint32_t (&x)[32]) {
+                    float m4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) m4[i] = fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 4]));
+#pragma unroll
+                    for (int i = 8; i < 32; i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) m4[k] = max3(m4[k], __uint_as_float(x[i + k]), __uint_as_float(x[i + k + 4]));
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                    if (__any_sync(0xffffffffu, mx > m + TC_TAU)) move_max(c, mx); // (m = -inf: any score)
+                    const float mm = m == -INFINITY ? 0.0f : -m;                   // nothing seen yet: weights 0
+                    const float2 sc2 = make_float2(sc, sc), mm2 = make_float2(mm, mm);
+                    uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
                         const float2 d = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc2, mm2);
@@ -397,8 +413,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                         p[i] = h2_pack(e.x, e.y);
                     }
                     tmem_st16(s_at + 16 * c, p);
+                };
+                uint32_t x[32], y[32];
+                tmem_ld32(s_at, x);
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
+                    wait_ld(x);
+                    tmem_ld32(s_at + 32 * c + 32, y);
+                    piece(c, x);
+                    wait_ld(y);
+                    if (c == 0) tmem_ld32(s_at + 64, x);
+                    piece(c + 1, y);
                 }
-                l += (la.x + la.y) + (lb.x + lb.y);
                 wait_st();
             }
             fence_before();
@@ -407,6 +433,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             n++;
         }
         // ---------------------------------------------------------------- the slot's output
+        float l = (la.x + la.y) + (lb.x + lb.y);
         if (ok && n > 0) {
             ok = __all_sync(0xffffffffu, wait(o_full + 8 * slot, 0));
             fence_after();
@@ -425,7 +452,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     for (int c = 0; c < D / 32; c++) {
                         uint32_t x[32];
                         tmem_ld32(o_at + 32 * c, x);
-                        wait_ld();
+                        wait_ld(x);
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
                             *reinterpret_cast<uint4*>(xo + row * (D + 4) + 32 * c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
@@ -453,7 +480,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 uint32_t x[32];
                 if (n > 0 && ok) {
                     tmem_ld32(o_at + 32 * c, x);
-                    wait_ld();
+                    wait_ld(x);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; i++) x[i] = ok ? 0u : 0x7FC00000u;
