@@ -6,8 +6,8 @@
 //   split   up to 128 rows (drafted tokens, short turns): both slots hold the same rows and take the key tiles in turn,
 //           each with its own running maximum, sum and output; merged at the end
 // Roles (16 warps of 128 registers, one block per SM): warps 0-3 and 4-7 the softmax of slots 0 and 1 (a thread per row),
-// warps 8-14 bring keys and values into shared memory (16-token units in turn: records dequantized, tail and new rows
-// converted; fp16), one thread of warp 15 issues the products:
+// warps 8-13 bring keys and values into shared memory (16-token units in turn: records dequantized, tail and new rows
+// converted; fp16), one thread of warps 14 and 15 issues the products of slots 0 and 1:
 //   S[128 x 128] = Q K'^T   (both from shared memory, K-major, 128-byte swizzle), fp32 in TMEM
 //   O[128 x D]  += P V      (P fp16 in TMEM over the first half of S's columns, V from shared memory, N-major)
 // K' = c ks + (kb - ref), fp16, ref = the key bias of the first finished page the block sees: the same shift of every
@@ -22,7 +22,7 @@
 
 namespace kush {
 
-constexpr int TC_TM = 256, TC_TN = 128, TC_THREADS = 16 * WARP, TC_NPROD = 7;
+constexpr int TC_TM = 256, TC_TN = 128, TC_THREADS = 16 * WARP, TC_NPROD = 6;
 constexpr float TC_TAU = 8.0f;
 
 __device__ int g_attend_error = 0;
@@ -202,6 +202,29 @@ __device__ __forceinline__ bool mbar_done(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok;
 }
+// the rest of a wait: the warp sleeps in try_wait for up to 20 us at a time (polls would take issue slots from the
+// softmax); 2 s without the phase and the block gives up
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    uint64_t t0 = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity), "r"(20000)
+            : "memory");
+        if (ok) return true;
+        if (*gave_up) return false;
+        uint64_t now;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+        if (t0 == 0) t0 = now;
+        else if (now - t0 > 2000000000ull) {
+            *gave_up = 1;
+            atomicExch(&g_attend_error, 1);
+            return false;
+        }
+    }
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -245,7 +268,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + M::MISC + 4);
     if (tid == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(sm + M::BARS);
-        const int count[7] = {8, 1, 8, 1, 1, 4, 1};
+        const int count[7] = {8, 2, 8, 2, 1, 4, 1};
         for (int i = 0; i < 14; i++) mbar_init(b + i, count[i / 2]);
         *gave_up = 0;
         fence_mbar_init();
@@ -254,26 +277,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    // bounded wait for a condition; false if this block gave up
-    auto until = [&](auto ready) -> bool {
-        uint64_t t0 = 0;
-        for (uint32_t n = 0;; n++) {
-            if (ready()) return true;
-            if (*gave_up) return false;
-            if (n % 64 == 0) {
-                uint64_t now;
-                asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-                if (t0 == 0) t0 = now;
-                else if (now - t0 > 2000000000ull) {
-                    *gave_up = 1;
-                    atomicExch(&g_attend_error, 1);
-                    return false;
-                }
-            }
-        }
-    };
-    // for the phase of `parity` of a barrier
-    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return until([&] { return mbar_done(bar, parity); }); };
+    // bounded wait for the phase of `parity` of a barrier; false if this block gave up
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return mbar_done(bar, parity) || wait_long(bar, parity, gave_up); };
     const int32_t* bt = a.block_table + int64_t(t.s) * a.max_pages;
     const uint8_t* hcache = a.cache + int64_t(h) * a.head_stride;
     const int full = t.ctx / P * P;                                                // cached tokens in finished pages
@@ -391,7 +396,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                         wait_st();
                     }
                 };
-                auto piece = [&](int c, const uint32_t (&x)[32]) {
+                auto top = [&](const uint32_t (&x)[32]) -> float {                 // the piece's largest score, log2 units
                     float m4[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) m4[i] = fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 4]));
@@ -399,32 +404,46 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     for (int i = 8; i < 32; i += 8)
 #pragma unroll
                         for (int k = 0; k < 4; k++) m4[k] = max3(m4[k], __uint_as_float(x[i + k]), __uint_as_float(x[i + k + 4]));
-                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                };
+                // the weights of piece c in place of its scores (first the differences, then all 32 exponentials without a
+                // dependence between them, under which the next piece's maximum is taken), its sum and its P
+                auto piece = [&](int c, uint32_t (&x)[32], uint32_t (&y)[32], float mx, auto last) -> float {
                     if (__any_sync(0xffffffffu, mx > m + TC_TAU)) move_max(c, mx); // (m = -inf: any score)
                     const float mm = m == -INFINITY ? 0.0f : -m;                   // nothing seen yet: weights 0
                     const float2 sc2 = make_float2(sc, sc), mm2 = make_float2(mm, mm);
+                    if constexpr (!decltype(last)::value) tmem_ld32(s_at + 32 * c + 32, y);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 d = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, mm2);
+                        x[i] = __float_as_uint(d.x);
+                        x[i + 1] = __float_as_uint(d.y);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = __float_as_uint(ex2(__uint_as_float(x[i])));
+                    float next = 0.0f;
+                    if constexpr (!decltype(last)::value) {
+                        wait_ld(y);
+                        next = top(y);
+                    }
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float2 d = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc2, mm2);
-                        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+                        const float2 e = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
                         if (i & 1) lb = __fadd2_rn(lb, e);
                         else la = __fadd2_rn(la, e);
                         p[i] = h2_pack(e.x, e.y);
                     }
                     tmem_st16(s_at + 16 * c, p);
+                    return next;
                 };
                 uint32_t x[32], y[32];
                 tmem_ld32(s_at, x);
-#pragma unroll 1
-                for (int c = 0; c < 4; c += 2) {
-                    wait_ld(x);
-                    tmem_ld32(s_at + 32 * c + 32, y);
-                    piece(c, x);
-                    wait_ld(y);
-                    if (c == 0) tmem_ld32(s_at + 64, x);
-                    piece(c + 1, y);
-                }
+                wait_ld(x);
+                float mx = piece(0, x, y, top(x), IC<0>{});
+                mx = piece(1, y, x, mx, IC<0>{});
+                mx = piece(2, x, y, mx, IC<0>{});
+                piece(3, y, x, mx, IC<1>{});
                 wait_st();
             }
             fence_before();
@@ -536,7 +555,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
 #pragma unroll
         for (int k = 0; k < 8; k++) rf8[k] = ref[8 * cc + k];
         // The stream of units x: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp's k-th is
-        // x = w + 7 k.  Where its units come from is worked out for 32 of them at a time, a lane each, which also asks for
+        // x = w + 6 k.  Where its units come from is worked out for 32 of them at a time, a lane each, which also asks for
         // their bytes into L2: a unit is then loaded into registers while the one before it is converted.
         const int units = 16 * (i1 - i0), w = wid - 8, mine = w < units ? (units - w + TC_NPROD - 1) / TC_NPROD : 0;
         auto batch = [&](int i, int32_t& f, int32_t& bl) {                         // token | kind, and the packed unit's block
@@ -707,78 +726,65 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             if (lane == 0) bar_arrive(bar_f);
         }
     } else {
-        // ---------------------------------------------------------------- the products, in the order of (tile, slot)
-        // S of a pair goes out before O of the pair before it when the slots differ, so that one slot's softmax runs under
-        // the other's products; a slot's own S has to wait for its O product, which reads P from S's columns.  The warp
-        // walks together on warp-uniform values (the products' operands live in uniform registers), one thread issues.
+        // ---------------------------------------------------------------- the products: a warp for each slot
+        // For each key tile S, then (P written) O: the next tile's S overwrites P, and products of one thread run in order.
+        // Two warps, because one thread's waits and issue (50 cycles a product) would leave the tensor cores idle for half
+        // the time; so one slot's products run under the other's.  The warp walks together on warp-uniform values (the
+        // products' operands live in uniform registers), one thread issues.
         constexpr uint32_t ID_S = instr_desc(128, TC_TN, false), ID_O = instr_desc(128, D, true);
         auto uni = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
         const bool leader = elect_one();
-        const uint32_t tm = uni(tmem);
-        const uint64_t q_desc = smem_desc(base + M::Q, 16, 1024), k_desc = smem_desc(base + M::K, 16, 1024);
-        const uint64_t v_desc = smem_desc(base + M::V, M::BLK, 1024);
-        const int n1 = uni(i1 - i0), e0 = uni(end0 - i0), g0 = uni(gap0 - i0), g1 = uni(gap1 - i0), pr = uni(paired);
-        auto works = [&](int slot, int n) -> bool {                                // active() of tile i0 + n
-            return pr ? (slot == 0 ? n < e0 : n < g0 || n >= g1) : (n & 1) == slot;
-        };
-        uint32_t done0 = 0, done1 = 0;                                             // O products issued per slot
-        int pn = -1, ps = 0;                                                       // the pair whose O product is due
-        int n = 0, slot = works(0, 0) ? 0 : 1;
-        while (ok && (n < n1 || pn >= 0)) {
-            const bool more = n < n1, s_first = pn < 0 || (more && slot != ps);
+        const int slot = uni(wid - 8 - TC_NPROD), n1 = uni(i1 - i0), pr = uni(paired);
+        // tiles this slot works on: paired, all but [skip0, skip1); split, every other one
+        const int skip0 = uni((slot == 0 ? end0 : gap0) - i0), skip1 = uni((slot == 0 ? i1 : gap1) - i0);
+        const uint32_t s_tm = uni(tmem) + 128 * slot, o_tm = s_tm + 256;
+        const uint64_t q_desc = smem_desc(base + M::Q + (pr && slot ? M::TILE : 0), 16, 1024);
+        const uint64_t k_desc = smem_desc(base + M::K, 16, 1024), v_desc = smem_desc(base + M::V, M::BLK, 1024);
+        uint32_t done = 0;                                                         // tiles done
 #pragma unroll 1
-            for (int step = 0; step < 2 && ok; step++) {
-                if ((step == 0) == s_first) {
-                    if (!more) continue;
-                    const int st = n & 1;
-                    ok = __all_sync(0xffffffffu, wait(k_full + 8 * st, (n >> 1) & 1));
-                    if (!ok) break;
-                    fence_after();
-                    if (leader) {
-                        const uint64_t qd = q_desc + (pr && slot ? M::TILE >> 4 : 0), kd = k_desc + st * (M::TILE >> 4);
+        for (int n = 0; n < n1; n++) {
+            const int st = n & 1;
+            const uint32_t full = (n >> 1) & 1;
+            const bool work = pr ? n < skip0 || n >= skip1 : (n & 1) == slot;
+            ok = __all_sync(0xffffffffu, wait(k_full + 8 * st, full));
+            if (!ok) break;
+            fence_after();
+            if (leader) {
+                if (work) {
+                    const uint64_t kd = k_desc + st * (M::TILE >> 4);
 #pragma unroll
-                        for (int k = 0; k < D / 16; k++) {
-                            const uint32_t off = ((k >> 2) * M::BLK + (k & 3) * 32) >> 4;
-                            mma_ss(tm + 128 * slot, qd + off, kd + off, ID_S, k > 0);
-                        }
-                        mma_commit(s_full + 8 * slot);
-                        if (slot == 1 || !works(1, n)) mma_commit(k_empty + 8 * st);
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint32_t off = ((k >> 2) * M::BLK + (k & 3) * 32) >> 4;
+                        mma_ss(s_tm, q_desc + off, kd + off, ID_S, k > 0);
                     }
-                    __syncwarp();
-                } else if (pn >= 0) {
-                    const int st = pn & 1;
-                    const uint32_t d = ps ? done1 : done0;
-                    ok = __all_sync(0xffffffffu, wait(v_full + 8 * st, (pn >> 1) & 1) && wait(p_full + 8 * ps, d & 1));
-                    if (!ok) break;
-                    fence_after();
-                    if (leader) {
-                        const uint64_t vd = v_desc + st * (M::TILE >> 4);
-#pragma unroll
-                        for (int k = 0; k < TC_TN / 16; k++)
-                            mma_ts(tm + 256 + 128 * ps, tm + 128 * ps + 8 * k, vd + k * (2048 >> 4), ID_O, d > 0 || k > 0);
-                        if (ps == 1 || !works(1, pn)) mma_commit(v_empty + 8 * st);
-                    }
-                    __syncwarp();
-                    if (ps) done1++;
-                    else done0++;
-                }
-            }
-            pn = more ? n : -1;
-            ps = slot;
-            if (more) {                                                            // the next active pair
-                if (slot == 0 && works(1, n)) {
-                    slot = 1;
+                    mma_commit(s_full + 8 * slot);
+                    mma_commit(k_empty + 8 * st);
                 } else {
-                    n++;
-                    slot = works(0, n) ? 0 : 1;
+                    bar_arrive(k_empty + 8 * st);
                 }
             }
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, wait(v_full + 8 * st, full) && (!work || wait(p_full + 8 * slot, done & 1)));
+            if (!ok) break;
+            fence_after();
+            if (leader) {
+                if (work) {
+                    const uint64_t vd = v_desc + st * (M::TILE >> 4);
+#pragma unroll
+                    for (int k = 0; k < TC_TN / 16; k++)
+                        mma_ts(o_tm, s_tm + 8 * k, vd + k * (2048 >> 4), ID_O, done > 0 || k > 0);
+                    mma_commit(v_empty + 8 * st);
+                } else {
+                    bar_arrive(v_empty + 8 * st);
+                }
+            }
+            __syncwarp();
+            done += work;
         }
-        // both slots' outputs; nothing of this block is in flight when it ends, whatever ended the loop
+        // the slot's output; nothing of this warp is in flight when the block ends, whatever ended the loop
         if (leader) {
-            mma_commit(o_full);
-            mma_commit(o_full + 8);
-            for (int i = 0; i < 1 << 20 && !(mbar_done(o_full, 0) && mbar_done(o_full + 8, 0)); i++) {
+            mma_commit(o_full + 8 * slot);
+            for (int i = 0; i < 1 << 20 && !mbar_done(o_full + 8 * slot, 0); i++) {
             }
         }
     }
