@@ -32,7 +32,7 @@ struct TcSmem {
     static constexpr int BLK = 128 * 128;                    // 128 rows x 64 channels of fp16: one swizzled block
     static constexpr int TILE = BLK * (D / 64);
     static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, REF = V + 2 * TILE;               // REF: fp32 [D]
-    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * 14, BYTES = MISC + 16 + 1024;          // + alignment
+    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * 15, BYTES = MISC + 16 + 1024;          // + alignment
     static_assert(BYTES <= 232448, "shared memory of a block");
 };
 
@@ -263,13 +263,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     float* ref = reinterpret_cast<float*>(sm + M::REF);
     const uint32_t bars = base + M::BARS;
     const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64,
-                   p_full = bars + 80, o_full = bars + 96;                         // pairs: [stage] or [slot]
+                   p_full = bars + 80, o_full = bars + 96, lead = bars + 112;      // pairs: [stage] or [slot]; slot 0's first weights
     volatile int* gave_up = reinterpret_cast<volatile int*>(sm + M::MISC);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + M::MISC + 4);
     if (tid == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(sm + M::BARS);
         const int count[7] = {8, 2, 8, 2, 1, 4, 1};
-        for (int i = 0; i < 14; i++) mbar_init(b + i, count[i / 2]);
+        for (int i = 0; i < 15; i++) mbar_init(b + i, i < 14 ? count[i / 2] : 1);
         *gave_up = 0;
         fence_mbar_init();
     }
@@ -449,8 +449,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(p_full + 8 * slot);
+            if (wid == 0 && lane == 0 && n == 0) bar_arrive(lead);
             n++;
         }
+        if (wid == 0 && lane == 0 && n == 0) bar_arrive(lead);                      // (slot 0 had no tile)
         // ---------------------------------------------------------------- the slot's output
         float l = (la.x + la.y) + (lb.x + lb.y);
         if (ok && n > 0) {
@@ -740,35 +742,39 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         const uint32_t s_tm = uni(tmem) + 128 * slot, o_tm = s_tm + 256;
         const uint64_t q_desc = smem_desc(base + M::Q + (pr && slot ? M::TILE : 0), 16, 1024);
         const uint64_t k_desc = smem_desc(base + M::K, 16, 1024), v_desc = smem_desc(base + M::V, M::BLK, 1024);
-        uint32_t done = 0;                                                         // tiles done
-#pragma unroll 1
-        for (int n = 0; n < n1; n++) {
-            const int st = n & 1;
-            const uint32_t full = (n >> 1) & 1;
-            const bool work = pr ? n < skip0 || n >= skip1 : (n & 1) == slot;
-            ok = __all_sync(0xffffffffu, wait(k_full + 8 * st, full));
-            if (!ok) break;
-            fence_after();
-            if (leader) {
-                if (work) {
-                    const uint64_t kd = k_desc + st * (M::TILE >> 4);
+        auto works = [&](int n) -> bool { return pr ? n < skip0 || n >= skip1 : (n & 1) == slot; };
+        auto scores = [&](int n) {                                                 // the leader: S of tile n (its keys are there)
+            if (works(n)) {
+                const uint64_t kd = k_desc + (n & 1) * (M::TILE >> 4);
 #pragma unroll
-                    for (int k = 0; k < D / 16; k++) {
-                        const uint32_t off = ((k >> 2) * M::BLK + (k & 3) * 32) >> 4;
-                        mma_ss(s_tm, q_desc + off, kd + off, ID_S, k > 0);
-                    }
-                    mma_commit(s_full + 8 * slot);
-                    mma_commit(k_empty + 8 * st);
-                } else {
-                    bar_arrive(k_empty + 8 * st);
+                for (int k = 0; k < D / 16; k++) {
+                    const uint32_t off = ((k >> 2) * M::BLK + (k & 3) * 32) >> 4;
+                    mma_ss(s_tm, q_desc + off, kd + off, ID_S, k > 0);
                 }
+                mma_commit(s_full + 8 * slot);
+                mma_commit(k_empty + 8 * (n & 1));
+            } else {
+                bar_arrive(k_empty + 8 * (n & 1));
             }
-            __syncwarp();
-            ok = __all_sync(0xffffffffu, wait(v_full + 8 * st, full) && (!work || wait(p_full + 8 * slot, done & 1)));
+        };
+        uint32_t done = 0;                                                         // tiles done
+        ok = __all_sync(0xffffffffu, wait(k_full, 0));
+        // Both softmaxes at once would leave the tensor cores idle, and then wait for them together: slot 1 starts half a
+        // period later, when slot 0 has its first weights, and stays there.
+        if (ok && slot == 1 && n1 >= 8) ok = __all_sync(0xffffffffu, wait(lead, 0));
+        fence_after();
+        if (leader && ok) scores(0);
+#pragma unroll 1
+        for (int n = 0; n < n1 && ok; n++) {
+            // the next keys are waited for before this tile's weights, so that S follows O at once
+            const int st = n & 1;
+            ok = wait(v_full + 8 * st, (n >> 1) & 1) && (n + 1 == n1 || wait(k_full + 8 * (st ^ 1), ((n + 1) >> 1) & 1)) &&
+                 (!works(n) || wait(p_full + 8 * slot, done & 1));
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after();
             if (leader) {
-                if (work) {
+                if (works(n)) {
                     const uint64_t vd = v_desc + st * (M::TILE >> 4);
 #pragma unroll
                     for (int k = 0; k < TC_TN / 16; k++)
@@ -777,9 +783,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 } else {
                     bar_arrive(v_empty + 8 * st);
                 }
+                if (n + 1 < n1) scores(n + 1);
             }
             __syncwarp();
-            done += work;
+            done += works(n);
         }
         // the slot's output; nothing of this warp is in flight when the block ends, whatever ended the loop
         if (leader) {
