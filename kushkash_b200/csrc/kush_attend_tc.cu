@@ -32,7 +32,7 @@ struct TcSmem {
     static constexpr int BLK = 128 * 128;                    // 128 rows x 64 channels of fp16: one swizzled block
     static constexpr int TILE = BLK * (D / 64);
     static constexpr int Q = 0, K = Q + 2 * TILE, V = K + 2 * TILE, REF = V + 2 * TILE;               // REF: fp32 [D]
-    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * 15, BYTES = MISC + 16 + 1024;          // + alignment
+    static constexpr int BARS = REF + 4 * D, MISC = BARS + 8 * 16, BYTES = MISC + 16 + 1024;          // + alignment
     static_assert(BYTES <= 232448, "shared memory of a block");
 };
 
@@ -263,13 +263,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     float* ref = reinterpret_cast<float*>(sm + M::REF);
     const uint32_t bars = base + M::BARS;
     const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64,
-                   p_full = bars + 80, o_full = bars + 96, lead = bars + 112;      // pairs: [stage] or [slot]; slot 0's first weights
+                   p_full = bars + 80, o_full = bars + 96, turn = bars + 112;      // pairs: [stage] or [slot]
     volatile int* gave_up = reinterpret_cast<volatile int*>(sm + M::MISC);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + M::MISC + 4);
     if (tid == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(sm + M::BARS);
-        const int count[7] = {8, 2, 8, 2, 1, 4, 1};
-        for (int i = 0; i < 15; i++) mbar_init(b + i, i < 14 ? count[i / 2] : 1);
+        const int count[8] = {8, 2, 8, 2, 1, 4, 1, 4};
+        for (int i = 0; i < 16; i++) mbar_init(b + i, count[i / 2]);
         *gave_up = 0;
         fence_mbar_init();
     }
@@ -338,11 +338,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         float m = -INFINITY;                                                       // the maximum in use, log2 units
         float2 la = make_float2(0.0f, 0.0f), lb = la;                              // the weights' sum, in four parts
         int n = 0;                                                                 // tiles done by this slot
+        // Paired slots take turns: both softmaxes at once would leave the tensor cores idle and then wait for them together.
+        // Slot 0's tile goes before slot 1's, slot 1's before slot 0's next; a tile that a slot has no part in passes on.
+        auto pass_on = [&] {
+            if (paired && lane == 0) bar_arrive(turn + 8 * slot);
+        };
         for (int it = i0; it < i1; it++) {
-            if (!active(slot, it)) continue;
-            ok = __all_sync(0xffffffffu, wait(s_full + 8 * slot, n & 1));           // (converged: tcgen05.ld is warp-aligned)
+            const int nt = it - i0;
+            const bool work = active(slot, it);
+            ok = !work || wait(s_full + 8 * slot, n & 1);
+            if (paired) ok = ok && (slot == 1 ? wait(turn, nt & 1) : nt == 0 || wait(turn + 8, (nt - 1) & 1));
+            ok = __all_sync(0xffffffffu, ok);                                      // (converged: tcgen05.ld is warp-aligned)
             if (!ok) break;
+            if (!work) {
+                pass_on();
+                continue;
+            }
             fence_after();
+            if (!busy) pass_on();
             if (busy) {
                 const int j0 = kt.tile(it) * TC_TN;
                 // columns [0, hi] seen, and of those [lo, ...) or [0, sk)
@@ -443,16 +456,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 float mx = piece(0, x, y, top(x), IC<0>{});
                 mx = piece(1, y, x, mx, IC<0>{});
                 mx = piece(2, x, y, mx, IC<0>{});
+                pass_on();
                 piece(3, y, x, mx, IC<1>{});
                 wait_st();
             }
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(p_full + 8 * slot);
-            if (wid == 0 && lane == 0 && n == 0) bar_arrive(lead);
             n++;
         }
-        if (wid == 0 && lane == 0 && n == 0) bar_arrive(lead);                      // (slot 0 had no tile)
         // ---------------------------------------------------------------- the slot's output
         float l = (la.x + la.y) + (lb.x + lb.y);
         if (ok && n > 0) {
@@ -759,9 +771,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         };
         uint32_t done = 0;                                                         // tiles done
         ok = __all_sync(0xffffffffu, wait(k_full, 0));
-        // Both softmaxes at once would leave the tensor cores idle, and then wait for them together: slot 1 starts half a
-        // period later, when slot 0 has its first weights, and stays there.
-        if (ok && slot == 1 && n1 >= 8) ok = __all_sync(0xffffffffu, wait(lead, 0));
         fence_after();
         if (leader && ok) scores(0);
 #pragma unroll 1
