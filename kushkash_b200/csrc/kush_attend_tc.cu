@@ -548,35 +548,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         fence_before();
     } else if (wid < 8 + TC_NPROD) {
         // ---------------------------------------------------------------- keys and values into shared memory
-        const int c = lane % U::LPR, rg = lane / U::LPR;
-        const IN* tail = static_cast<const IN*>(a.tail_k) + (int64_t(a.tail_idx[t.s]) * a.H + h) * P * D;
-        const IN* kn = static_cast<const IN*>(a.k_new) + t.q0 * a.k_stride + int64_t(h) * D;
-        const IN* vn = static_cast<const IN*>(a.v_new) + t.q0 * a.v_stride + int64_t(h) * D;
-        // the lane's two chunks, in the order of its stores (int8: lanes of a row's second block store their odd chunk
-        // first, so that the eight lanes of a row fall in distinct banks)
-        const int swap = BITS == 8 && D == 128 ? c >> 2 : 0;
-        const int c_a = BITS == 4 ? c : 2 * c + swap, c_b = BITS == 4 ? c + D / 16 : 2 * c + 1 - swap;
-        const uint32_t at_a = tile_off(rg, c_a), at_b = tile_off(rg, c_b);         // in a unit's first rows
-        uint32_t rf[8];                                                            // the reference of the lane's channels
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            rf[i] = h2_pack(ref[8 * c_a + 2 * i], ref[8 * c_a + 2 * i + 1]);
-            rf[4 + i] = h2_pack(ref[8 * c_b + 2 * i], ref[8 * c_b + 2 * i + 1]);
-        }
-        constexpr int RPI = WARP / CH, NI = 16 / RPI;                              // unpacked rows: rows per step, steps
-        const int cc = lane % CH, r0 = lane / CH;
-        float rf8[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) rf8[k] = ref[8 * cc + k];
-        // The stream of units x: 8 of a tile's keys, 8 of its values, the next tile's keys, ...; this warp's k-th is
+        // Work comes in units of 16 tokens, keys and values: 8 of a tile, then the next tile's; this warp's k-th unit is
         // x = w + 6 k.  Where its units come from is worked out for 32 of them at a time, a lane each, which also asks for
-        // their bytes into L2: a unit is then loaded into registers while the one before it is converted.
-        const int units = 16 * (i1 - i0), w = wid - 8, mine = w < units ? (units - w + TC_NPROD - 1) / TC_NPROD : 0;
+        // their bytes into L2.  A unit's keys are converted, then the next unit's keys loaded into the same registers, under
+        // the conversion of the values, and the other way round.
+        const int units = 8 * (i1 - i0), w = wid - 8, mine = w < units ? (units - w + TC_NPROD - 1) / TC_NPROD : 0;
         auto batch = [&](int i, int32_t& f, int32_t& bl) {                         // token | kind, and the packed unit's block
             const int k = 32 * i + lane, x = w + TC_NPROD * k;
             f = bl = 0;
             if (k < mine) {
-                const int j0 = kt.tile(i0 + (x >> 4)) * TC_TN + 16 * (x & 7);
+                const int j0 = kt.tile(i0 + (x >> 3)) * TC_TN + 16 * (x & 7);
                 // 0 no row sees a token of it, 1 packed, 2 new rows, 3 mixed
                 const int kind = j0 > t.p1 || (j0 + 15 < kt.lo && j0 >= kt.ns) ? 0 : j0 + 16 <= full ? 1
                                  : j0 >= t.ctx && j0 + 15 <= t.p1 ? 2 : 3;
@@ -584,160 +565,181 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 if (kind == 1) {
                     bl = bt[j0 / P];
                     const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
-                    bulk_to_l2(rec + (x & 8 ? F::OFF_VQ : 0) + j0 % P * F::DC, 16 * F::DC);
-                    if (j0 % P == 0 && !(x & 8)) bulk_to_l2(rec + F::OFF_KS, F::RB - F::OFF_KS);
+                    if constexpr (P == 16) {
+                        bulk_to_l2(rec, F::RB);
+                    } else {
+                        bulk_to_l2(rec + j0 % P * F::DC, 16 * F::DC);
+                        bulk_to_l2(rec + F::OFF_VQ + j0 % P * F::DC, 16 * F::DC);
+                        bulk_to_l2(rec + F::OFF_KS, F::RB - F::OFF_KS);
+                    }
                 }
             }
         };
         int32_t from, blk, from1, blk1;                                            // of units 32 i + lane; of the next batch
         batch(0, from, blk);
         batch(1, from1, blk1);
-        // a row of an unpacked unit (new rows, the unfinished page, unseen tokens): 16 bytes of row i * RPI + r0
-        auto unpacked = [&](bool kv, int j0, int kind, int i) -> uint4 {
-            const int j = j0 + i * RPI + r0;
-            const IN* src = nullptr;
-            if (kind == 2 || (kind == 3 && j >= t.ctx && kt.seen(j, t.p1)))
-                src = kv ? vn + int64_t(j - t.ctx) * a.v_stride : kn + int64_t(j - t.ctx) * a.k_stride;
-            else if (kind == 3 && !kv && j >= full && kt.seen(j, t.p1))
-                src = tail + (j % P) * D;
-            return src ? *reinterpret_cast<const uint4*>(src + 8 * cc) : make_uint4(0, 0, 0, 0);
-        };
-        // What is fetched into registers for this warp's next unit: an unpacked unit's rows; a packed one's codes (words
-        // [0, RPL W)) and, for keys, its scales and biases of chunks a and b (words [16, 32)), for values the scale of row
-        // lane or the bias of row lane - 16 (word 16).
-        constexpr int NRAW = NI < 8 ? 8 : NI;
-        uint4 raw[NRAW];
-        uint32_t* const rw = reinterpret_cast<uint32_t*>(raw);
-        auto fetch = [&](int k) -> int32_t {                                       // returns its first token | kind
-            if (k >= mine) return 1;
-            if ((k & 31) == 0 && k > 0) {
-                from = from1;
-                blk = blk1;
-                batch(k / 32 + 1, from1, blk1);
-            }
-            const int32_t f = __shfl_sync(0xffffffffu, from, k & 31), bl = __shfl_sync(0xffffffffu, blk, k & 31);
-            const int x = w + TC_NPROD * k, j0 = f & ~15;
-            const bool kv = x & 8;
-            if ((f & 15) != 1) {
+
+        // packed: lane = (row group rg, column c) has rows rg, rg + RG, ... and the chunks c_a, c_b of each, in the order of
+        // its stores (int8: lanes of a row's second block store their odd chunk first, so that the eight lanes of a row fall
+        // in distinct banks)
+        const int c = lane % U::LPR, rg = lane / U::LPR;
+        const int swap = BITS == 8 && D == 128 ? c >> 2 : 0;
+        const int c_a = BITS == 4 ? c : 2 * c + swap, c_b = BITS == 4 ? c + D / 16 : 2 * c + 1 - swap;
+        const uint32_t at_a = tile_off(rg, c_a), at_b = tile_off(rg, c_b);         // in a unit's first rows
+        const int code_a = rg * F::DC + (BITS == 4 ? 8 * c : 8 * c_a), code_b = rg * F::DC + 8 * c_b;
+        uint32_t rf[8];                                                            // the reference of the lane's channels
 #pragma unroll
-                for (int i = 0; i < NI; i++) raw[i] = unpacked(kv, j0, f & 15, i);
-                return f;
-            }
-            const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
-            const uint8_t* rows = rec + (kv ? F::OFF_VQ : 0) + (j0 % P + rg) * F::DC;
-#pragma unroll
-            for (int i = 0; i < U::RPL; i++) {
-                if constexpr (BITS == 4) {
-                    load_words(rows + U::RG * i * F::DC + 8 * c, rw + 2 * i, 2);
-                } else if constexpr (D == 128) {                                   // the two halves in the order of the stores
-                    load_words(rows + U::RG * i * F::DC + 8 * c_a, rw + 4 * i, 2);
-                    load_words(rows + U::RG * i * F::DC + 8 * c_b, rw + 4 * i + 2, 2);
-                } else {
-                    load_words(rows + U::RG * i * F::DC + 16 * c, rw + 4 * i, 4);
-                }
-            }
-            if (kv) {
-                rw[16] = reinterpret_cast<const uint16_t*>(rec + (lane < 16 ? F::OFF_VS : F::OFF_VB))[j0 % P + (lane & 15)];
-            } else {
-                raw[4] = *reinterpret_cast<const uint4*>(rec + F::OFF_KS + 16 * c_a);
-                raw[5] = *reinterpret_cast<const uint4*>(rec + F::OFF_KS + 16 * c_b);
-                raw[6] = *reinterpret_cast<const uint4*>(rec + F::OFF_KB + 16 * c_a);
-                raw[7] = *reinterpret_cast<const uint4*>(rec + F::OFF_KB + 16 * c_b);
-            }
-            return f;
-        };
-        auto store_row = [&](uint32_t dst, int i, const uint32_t (&lo)[4], const uint32_t (&hi)[4]) {
-            const uint32_t flip = U::RG == 4 && (i & 1) ? 64 : 0;                  // rows 4 apart: the swizzle's bit 2
-            st_chunk(dst + ((at_a ^ flip) + U::RG * 128 * i), lo[0], lo[1], lo[2], lo[3]);
-            st_chunk(dst + ((at_b ^ flip) + U::RG * 128 * i), hi[0], hi[1], hi[2], hi[3]);
-        };
-        int32_t f = fetch(0);
-        for (int k = 0; k < mine && ok; k++) {
-            const int x = w + TC_NPROD * k, n = x >> 4, st = n & 1, u = x & 7, j0 = f & ~15, kind = f & 15;
-            const bool kv = x & 8;
-            const uint32_t dst = base + (kv ? M::V : M::K) + st * M::TILE + u * 2048;
-            const uint32_t bar_e = (kv ? v_empty : k_empty) + 8 * st, bar_f = (kv ? v_full : k_full) + 8 * st;
+        for (int i = 0; i < 4; i++) {
+            rf[i] = h2_pack(ref[8 * c_a + 2 * i], ref[8 * c_a + 2 * i + 1]);
+            rf[4 + i] = h2_pack(ref[8 * c_b + 2 * i], ref[8 * c_b + 2 * i + 1]);
+        }
+        // unpacked (new rows, the unfinished page, unseen tokens): chunk cc of rows r0, r0 + RPI, ...
+        constexpr int RPI = WARP / CH, NI = 16 / RPI;
+        const int cc = lane % CH, r0 = lane / CH;
+        const IN* tail = static_cast<const IN*>(a.tail_k) + (int64_t(a.tail_idx[t.s]) * a.H + h) * P * D + 8 * cc;
+        const IN* kn = static_cast<const IN*>(a.k_new) + t.q0 * a.k_stride + int64_t(h) * D + 8 * cc;
+        const IN* vn = static_cast<const IN*>(a.v_new) + t.q0 * a.v_stride + int64_t(h) * D + 8 * cc;
+
+        // registers of a unit's keys (values): packed, words [0, RPL W) codes and [16, 32) scales and biases of chunks a and
+        // b (word 16: the scale of row lane or the bias of row lane - 16); unpacked, the rows
+        uint32_t kr[32], vr[32];
+        auto load = [&](auto kvc, int32_t f, int32_t bl, uint32_t (&r)[32]) {
+            constexpr bool kv = decltype(kvc)::value;
+            const int j0 = f & ~15, kind = f & 15;
             if (kind == 1) {
-                uint32_t cw[U::RPL][U::W], sb[16];
+                const uint8_t* rec = hcache + int64_t(bl) * a.block_stride;
+                const uint8_t* rows = rec + (kv ? F::OFF_VQ : 0) + j0 % P * F::DC;
 #pragma unroll
-                for (int i = 0; i < U::RPL * U::W; i++) cw[i / U::W][i % U::W] = rw[i];
+                for (int i = 0; i < U::RPL; i++) {
+                    load_words(rows + code_a + U::RG * i * F::DC, r + U::W * i, 2);
+                    if constexpr (BITS == 8) load_words(rows + code_b + U::RG * i * F::DC, r + U::W * i + 2, 2);
+                }
+                if constexpr (kv) {
+                    r[16] = reinterpret_cast<const uint16_t*>(rec + (lane < 16 ? F::OFF_VS : F::OFF_VB))[j0 % P + (lane & 15)];
+                } else {
+                    load_words(rec + F::OFF_KS + 16 * c_a, r + 16, 4);
+                    load_words(rec + F::OFF_KS + 16 * c_b, r + 20, 4);
+                    load_words(rec + F::OFF_KB + 16 * c_a, r + 24, 4);
+                    load_words(rec + F::OFF_KB + 16 * c_b, r + 28, 4);
+                }
+                return;
+            }
 #pragma unroll
-                for (int i = 0; i < 16; i++) sb[i] = rw[16 + i];
-                f = fetch(k + 1);
-                ok = wait(bar_e, ((n >> 1) - 1) & 1);                              // (a fresh barrier lets tiles 0 and 1 pass)
-                if (kv) {
+            for (int i = 0; i < NI; i++) {
+                const int j = j0 + i * RPI + r0;
+                const IN* src = nullptr;
+                if (kind == 2 || (kind == 3 && j >= t.ctx && kt.seen(j, t.p1)))
+                    src = kv ? vn + int64_t(j - t.ctx) * a.v_stride : kn + int64_t(j - t.ctx) * a.k_stride;
+                else if (!kv && kind == 3 && j >= full && kt.seen(j, t.p1))
+                    src = tail + (j % P) * D;
+                const uint4 v = src ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+                r[4 * i] = v.x;
+                r[4 * i + 1] = v.y;
+                r[4 * i + 2] = v.z;
+                r[4 * i + 3] = v.w;
+            }
+        };
+        auto convert = [&](auto kvc, int32_t f, uint32_t (&r)[32], uint32_t dst) {
+            constexpr bool kv = decltype(kvc)::value;
+            const int j0 = f & ~15, kind = f & 15;
+            if (kind == 1) {
+                if constexpr (!kv) {
 #pragma unroll
-                    for (int i = 0; i < U::RPL; i++) {
-                        uint32_t lo[4], hi[4];
-                        codes_of<BITS>(cw[i], lo, hi);
-                        const int row = rg + U::RG * i;
-                        const uint32_t vs = __shfl_sync(0xffffffffu, sb[0], row) * 0x10001u;
-                        const uint32_t vb = __shfl_sync(0xffffffffu, sb[0], 16 + row) * 0x10001u;
+                    for (int i = 0; i < 8; i++) r[24 + i] = h2_sub_u(r[24 + i], rf[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < U::RPL; i++) {
+                    uint32_t cw[U::W], lo[4], hi[4];
+#pragma unroll
+                    for (int j = 0; j < U::W; j++) cw[j] = r[U::W * i + j];
+                    codes_of<BITS>(cw, lo, hi);
+                    if constexpr (kv) {
+                        const uint32_t vs = __shfl_sync(0xffffffffu, r[16], rg + U::RG * i) * 0x10001u;
+                        const uint32_t vb = __shfl_sync(0xffffffffu, r[16], 16 + rg + U::RG * i) * 0x10001u;
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             lo[j] = h2_fma_u(lo[j], vs, vb);
                             hi[j] = h2_fma_u(hi[j], vs, vb);
                         }
-                        store_row(dst, i, lo, hi);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sb[8 + i] = h2_sub_u(sb[8 + i], rf[i]);
-#pragma unroll
-                    for (int i = 0; i < U::RPL; i++) {
-                        uint32_t lo[4], hi[4];
-                        codes_of<BITS>(cw[i], lo, hi);
+                    } else {
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            lo[j] = h2_fma_u(lo[j], sb[j], sb[8 + j]);
-                            hi[j] = h2_fma_u(hi[j], sb[4 + j], sb[12 + j]);
+                            lo[j] = h2_fma_u(lo[j], r[16 + j], r[24 + j]);
+                            hi[j] = h2_fma_u(hi[j], r[20 + j], r[28 + j]);
                         }
-                        store_row(dst, i, lo, hi);
                     }
+                    const uint32_t flip = U::RG == 4 && (i & 1) ? 64 : 0;          // rows 4 apart: the swizzle's bit 2
+                    st_chunk(dst + ((at_a ^ flip) + U::RG * 128 * i), lo[0], lo[1], lo[2], lo[3]);
+                    st_chunk(dst + ((at_b ^ flip) + U::RG * 128 * i), hi[0], hi[1], hi[2], hi[3]);
                 }
-            } else {
-                // convert a row, then fetch the same row of this warp's next unit if that is unpacked too (a new batch waits)
-                ok = wait(bar_e, ((n >> 1) - 1) & 1);
-                const int32_t fn = __shfl_sync(0xffffffffu, from, (k + 1) & 31);
-                const int xn = x + TC_NPROD, jn = fn & ~15, kindn = fn & 15;
-                const bool again = k + 1 < mine && kindn != 1 && ((k + 1) & 31) != 0;
-#pragma unroll
-                for (int i = 0; i < NI; i++) {
-                    const int row = i * RPI + r0, j = j0 + row;
-                    const IN* e = reinterpret_cast<const IN*>(&raw[i]);
-                    const bool sub = !kv && (kind == 2 || (kind == 3 && kt.seen(j, t.p1)));
-                    uint32_t p[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        p[k] = h2_pack(to_f32(e[2 * k]) - (sub ? rf8[2 * k] : 0.0f), to_f32(e[2 * k + 1]) - (sub ? rf8[2 * k + 1] : 0.0f));
-                    st_chunk(dst + tile_off(row, cc), p[0], p[1], p[2], p[3]);
-                    if (again) raw[i] = unpacked(xn & 8, jn, kindn, i);
-                }
-                f = again ? fn : fetch(k + 1);
-                if (kind == 3) {                                                   // its cached tokens, one row after the other
-#pragma unroll 1
-                    for (int i = 0; i < NI; i++) {
-                        const int row = i * RPI + r0, j = j0 + row;
-                        if (!kt.seen(j, t.p1) || j >= (kv ? t.ctx : full)) continue;
-                        const uint8_t* rec = hcache + int64_t(bt[j / P]) * a.block_stride;
-                        const int at = j % P;
-                        float y[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const int d = 8 * cc + k;
-                            y[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + at * F::DC, d)), h_load(rec + F::OFF_VS, at),
-                                             h_load(rec + F::OFF_VB, at))
-                                      : fmaf(float(code_at<D, BITS>(rec + at * F::DC, d)), h_load(rec + F::OFF_KS, d),
-                                             h_load(rec + F::OFF_KB, d)) - rf8[k];
-                        }
-                        st_chunk(dst + tile_off(row, cc), h2_pack(y[0], y[1]), h2_pack(y[2], y[3]), h2_pack(y[4], y[5]),
-                                 h2_pack(y[6], y[7]));
-                    }
-                }
+                return;
             }
+            const float4 ra = *reinterpret_cast<const float4*>(ref + 8 * cc), rb = *reinterpret_cast<const float4*>(ref + 8 * cc + 4);
+            const float rf8[8] = {ra.x, ra.y, ra.z, ra.w, rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int row = i * RPI + r0;
+                const IN* e = reinterpret_cast<const IN*>(r + 4 * i);
+                const bool sub = !kv && (kind == 2 || (kind == 3 && kt.seen(j0 + row, t.p1)));
+                uint32_t p[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    p[k] = kv ? h2_pack(to_f32(e[2 * k]), to_f32(e[2 * k + 1]))
+                              : h2_pack(to_f32(e[2 * k]) - (sub ? rf8[2 * k] : 0.0f), to_f32(e[2 * k + 1]) - (sub ? rf8[2 * k + 1] : 0.0f));
+                st_chunk(dst + tile_off(row, cc), p[0], p[1], p[2], p[3]);
+            }
+            if (kind != 3) return;
+#pragma unroll 1
+            for (int i = 0; i < NI; i++) {                                         // its cached tokens, one row after the other
+                const int row = i * RPI + r0, j = j0 + row;
+                if (!kt.seen(j, t.p1) || j >= (kv ? t.ctx : full)) continue;
+                const uint8_t* rec = hcache + int64_t(bt[j / P]) * a.block_stride;
+                const int at = j % P;
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int d = 8 * cc + k;
+                    y[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + at * F::DC, d)), h_load(rec + F::OFF_VS, at),
+                                     h_load(rec + F::OFF_VB, at))
+                              : fmaf(float(code_at<D, BITS>(rec + at * F::DC, d)), h_load(rec + F::OFF_KS, d),
+                                     h_load(rec + F::OFF_KB, d)) - rf8[k];
+                }
+                st_chunk(dst + tile_off(row, cc), h2_pack(y[0], y[1]), h2_pack(y[2], y[3]), h2_pack(y[4], y[5]), h2_pack(y[6], y[7]));
+            }
+        };
+        int32_t f = __shfl_sync(0xffffffffu, from, 0), bl = __shfl_sync(0xffffffffu, blk, 0);
+        if (mine > 0) {
+            load(IC<0>{}, f, bl, kr);
+            load(IC<1>{}, f, bl, vr);
+        }
+#pragma unroll 1
+        for (int k = 0; k < mine && ok; k++) {
+            const int x = w + TC_NPROD * k, n = x >> 3, st = n & 1;
+            const uint32_t dst = base + M::K + st * M::TILE + (x & 7) * 2048, before = ((n >> 1) - 1) & 1;
+            int32_t f1 = 0, bl1 = 0;
+            if (k + 1 < mine) {
+                if (((k + 1) & 31) == 0) {
+                    from = from1;
+                    blk = blk1;
+                    batch((k + 1) / 32 + 1, from1, blk1);
+                }
+                f1 = __shfl_sync(0xffffffffu, from, (k + 1) & 31);
+                bl1 = __shfl_sync(0xffffffffu, blk, (k + 1) & 31);
+            }
+            ok = wait(k_empty + 8 * st, before);                                   // (a fresh barrier lets tiles 0 and 1 pass)
+            convert(IC<0>{}, f, kr, dst);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(k_full + 8 * st);
+            if (k + 1 < mine) load(IC<0>{}, f1, bl1, kr);
+            ok = ok && wait(v_empty + 8 * st, before);
+            convert(IC<1>{}, f, vr, dst + (M::V - M::K));
             fence_async();
             ok = __all_sync(0xffffffffu, ok);
-            if (lane == 0) bar_arrive(bar_f);
+            if (lane == 0) bar_arrive(v_full + 8 * st);
+            if (k + 1 < mine) load(IC<1>{}, f1, bl1, vr);
+            f = f1;
+            bl = bl1;
         }
     } else {
         // ---------------------------------------------------------------- the products: a warp for each slot
