@@ -258,6 +258,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         return;
     }
     const bool paired = t.nr > 128;
+    // softmax warps with rows, of slot 0 and 1; the others join the producers
+    const int rows0 = (min(t.nr, 128) + WARP - 1) / WARP, rows1 = paired ? (t.nr - 128 + WARP - 1) / WARP : rows0;
+    const int n_prod = TC_NPROD + 8 - rows0 - rows1;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* sm = smem_raw + (base - smem_u32(smem_raw));
     float* ref = reinterpret_cast<float*>(sm + M::REF);
@@ -268,8 +271,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + M::MISC + 4);
     if (tid == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(sm + M::BARS);
-        const int count[8] = {8, 2, 8, 2, 1, 4, 1, 4};
-        for (int i = 0; i < 16; i++) mbar_init(b + i, count[i / 2]);
+        const int count[8] = {8, 2, 8, 2, 1, 0, 1, 0};                             // (0: a slot's warps)
+        for (int i = 0; i < 16; i++) mbar_init(b + i, count[i / 2] ? count[i / 2] : i & 1 ? rows1 : rows0);
         *gave_up = 0;
         fence_mbar_init();
     }
@@ -325,11 +328,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     };
     bool ok = true;
 
-    if (wid < 8) {
+    if (wid < 8 && (wid & 3) < (wid < 4 ? rows0 : rows1)) {
         // ---------------------------------------------------------------- softmax: thread = row of its slot
         const int slot = wid >> 2, row = (wid & 3) * WARP + lane, wrow = (wid & 3) * WARP;
         const int r = paired ? slot * 128 + row : row;                             // tile row
-        const bool busy = (paired ? slot * 128 : 0) + wrow < t.nr;                 // this warp has rows
         const int pos = t.ctx + (t.r0 + min(r, t.nr - 1)) / a.G;
         const int wp0 = __shfl_sync(0xffffffffu, pos, 0), wp1 = __shfl_sync(0xffffffffu, pos, 31);
         const float sc = fmaxf(fabsf(a.sm_log2), 1e-30f);                          // (a masked score stays -inf under scale 0)
@@ -355,8 +357,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 continue;
             }
             fence_after();
-            if (!busy) pass_on();
-            if (busy) {
+            {
                 const int j0 = kt.tile(it) * TC_TN;
                 // columns [0, hi] seen, and of those [lo, ...) or [0, sk)
                 const int hi = pos - j0, lo = a.window > 0 ? pos - a.window + 1 - j0 : -1, sk = a.sinks - j0;
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         if (!paired) {
             // both slots' products are done before the key buffers are reused
             if (ok && slot == 1) ok = __all_sync(0xffffffffu, wait(o_full, 0));
-            if (slot == 1 && busy) {
+            if (slot == 1) {
                 xm[row] = n > 0 ? m : -INFINITY;
                 xm[128 + row] = l;
                 if (n > 0 && ok) {
@@ -492,9 +493,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     }
                 }
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"r"(2 * WARP * rows0) : "memory");
         }
-        if (busy && (paired || slot == 0)) {
+        if (paired || slot == 0) {
             float mo = -INFINITY, f0 = 1.0f, f1 = 0.0f;
             if (!paired) {
                 mo = xm[row];
@@ -546,15 +547,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             }
         }
         fence_before();
-    } else if (wid < 8 + TC_NPROD) {
+    } else if (wid < 8 + TC_NPROD) {                                               // (and softmax warps without rows)
         // ---------------------------------------------------------------- keys and values into shared memory
         // Work comes in units of 16 tokens, keys and values: 8 of a tile, then the next tile's; this warp's k-th unit is
-        // x = w + 6 k.  Where its units come from is worked out for 32 of them at a time, a lane each, which also asks for
+        // x = w + n_prod k.  Where its units come from is worked out for 32 of them at a time, a lane each, which also asks for
         // their bytes into L2.  A unit's keys are converted, then the next unit's keys loaded into the same registers, under
         // the conversion of the values, and the other way round.
-        const int units = 8 * (i1 - i0), w = wid - 8, mine = w < units ? (units - w + TC_NPROD - 1) / TC_NPROD : 0;
+        const int w = wid >= 8 ? wid - 8 : TC_NPROD + (wid < 4 ? wid - rows0 : 4 - rows0 + (wid & 3) - rows1);
+        const int units = 8 * (i1 - i0), mine = w < units ? (units - w + n_prod - 1) / n_prod : 0;
         auto batch = [&](int i, int32_t& f, int32_t& bl) {                         // token | kind, and the packed unit's block
-            const int k = 32 * i + lane, x = w + TC_NPROD * k;
+            const int k = 32 * i + lane, x = w + n_prod * k;
             f = bl = 0;
             if (k < mine) {
                 const int j0 = kt.tile(i0 + (x >> 3)) * TC_TN + 16 * (x & 7);
@@ -714,7 +716,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         }
 #pragma unroll 1
         for (int k = 0; k < mine && ok; k++) {
-            const int x = w + TC_NPROD * k, n = x >> 3, st = n & 1;
+            const int x = w + n_prod * k, n = x >> 3, st = n & 1;
             const uint32_t dst = base + M::K + st * M::TILE + (x & 7) * 2048, before = ((n >> 1) - 1) & 1;
             int32_t f1 = 0, bl1 = 0;
             if (k + 1 < mine) {
