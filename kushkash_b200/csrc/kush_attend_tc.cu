@@ -595,15 +595,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             rf[i] = h2_pack(ref[8 * c_a + 2 * i], ref[8 * c_a + 2 * i + 1]);
             rf[4 + i] = h2_pack(ref[8 * c_b + 2 * i], ref[8 * c_b + 2 * i + 1]);
         }
-        // unpacked (new rows, the unfinished page, unseen tokens): chunk cc of rows r0, r0 + RPI, ...
+        // new rows: chunk cc of rows r0, r0 + RPI, ...
         constexpr int RPI = WARP / CH, NI = 16 / RPI;
         const int cc = lane % CH, r0 = lane / CH;
-        const IN* tail = static_cast<const IN*>(a.tail_k) + (int64_t(a.tail_idx[t.s]) * a.H + h) * P * D + 8 * cc;
-        const IN* kn = static_cast<const IN*>(a.k_new) + t.q0 * a.k_stride + int64_t(h) * D + 8 * cc;
-        const IN* vn = static_cast<const IN*>(a.v_new) + t.q0 * a.v_stride + int64_t(h) * D + 8 * cc;
+        const uint32_t at_r = tile_off(r0, cc);
 
         // registers of a unit's keys (values): packed, words [0, RPL W) codes and [16, 32) scales and biases of chunks a and
-        // b (word 16: the scale of row lane or the bias of row lane - 16); unpacked, the rows
+        // b (word 16: the scale of row lane or the bias of row lane - 16); new rows, the rows
         uint32_t kr[32], vr[32];
         auto load = [&](auto kvc, int32_t f, int32_t bl, uint32_t (&r)[32]) {
             constexpr bool kv = decltype(kvc)::value;
@@ -626,19 +624,49 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 }
                 return;
             }
+            if (kind != 2) return;
+            const int64_t stride = kv ? a.v_stride : a.k_stride;
+            const IN* src = static_cast<const IN*>(kv ? a.v_new : a.k_new) + (t.q0 + (j0 - t.ctx + r0)) * stride + int64_t(h) * D + 8 * cc;
 #pragma unroll
+            for (int i = 0; i < NI; i++, src += RPI * stride) load_words(reinterpret_cast<const uint8_t*>(src), r + 4 * i, 4);
+        };
+        // a unit that is not of one kind (the unfinished page, its border to the new rows, tokens that no row sees, which are
+        // zeros): row after row
+        auto mixed = [&](auto kvc, int j0, int kind, uint32_t dst) {
+            constexpr bool kv = decltype(kvc)::value;
+            const int64_t stride = kv ? a.v_stride : a.k_stride;
+            const IN* rows = static_cast<const IN*>(kv ? a.v_new : a.k_new) + (t.q0 + (j0 - t.ctx)) * stride + int64_t(h) * D + 8 * cc;
+            const IN* tail = static_cast<const IN*>(a.tail_k) + (int64_t(a.tail_idx[t.s]) * a.H + h) * P * D + 8 * cc;
+#pragma unroll 1
             for (int i = 0; i < NI; i++) {
-                const int j = j0 + i * RPI + r0;
-                const IN* src = nullptr;
-                if (kind == 2 || (kind == 3 && j >= t.ctx && kt.seen(j, t.p1)))
-                    src = kv ? vn + int64_t(j - t.ctx) * a.v_stride : kn + int64_t(j - t.ctx) * a.k_stride;
-                else if (!kv && kind == 3 && j >= full && kt.seen(j, t.p1))
-                    src = tail + (j % P) * D;
-                const uint4 v = src ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-                r[4 * i] = v.x;
-                r[4 * i + 1] = v.y;
-                r[4 * i + 2] = v.z;
-                r[4 * i + 3] = v.w;
+                const int row = i * RPI + r0, j = j0 + row;
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) y[k] = 0.0f;
+                if (kind == 3 && kt.seen(j, t.p1)) {
+                    if (j >= t.ctx || (!kv && j >= full)) {
+                        const uint4 raw = *reinterpret_cast<const uint4*>(j >= t.ctx ? rows + row * stride : tail + (j % P) * D);
+                        const IN* e = reinterpret_cast<const IN*>(&raw);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) y[k] = to_f32(e[k]);
+                    } else {
+                        const uint8_t* rec = hcache + int64_t(bt[j / P]) * a.block_stride;
+                        const int at = j % P;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const int d = 8 * cc + k;
+                            y[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + at * F::DC, d)), h_load(rec + F::OFF_VS, at),
+                                             h_load(rec + F::OFF_VB, at))
+                                      : fmaf(float(code_at<D, BITS>(rec + at * F::DC, d)), h_load(rec + F::OFF_KS, d),
+                                             h_load(rec + F::OFF_KB, d));
+                        }
+                    }
+                    if constexpr (!kv) {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) y[k] -= ref[8 * cc + k];
+                    }
+                }
+                st_chunk(dst + tile_off(row, cc), h2_pack(y[0], y[1]), h2_pack(y[2], y[3]), h2_pack(y[4], y[5]), h2_pack(y[6], y[7]));
             }
         };
         auto convert = [&](auto kvc, int32_t f, uint32_t (&r)[32], uint32_t dst) {
@@ -676,37 +704,29 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 }
                 return;
             }
+            if (kind != 2) {
+                mixed(kvc, j0, kind, dst);
+                return;
+            }
             const float4 ra = *reinterpret_cast<const float4*>(ref + 8 * cc), rb = *reinterpret_cast<const float4*>(ref + 8 * cc + 4);
-            const float rf8[8] = {ra.x, ra.y, ra.z, ra.w, rb.x, rb.y, rb.z, rb.w};
+            const float2 minus[4] = {make_float2(-ra.x, -ra.y), make_float2(-ra.z, -ra.w), make_float2(-rb.x, -rb.y), make_float2(-rb.z, -rb.w)};
 #pragma unroll
             for (int i = 0; i < NI; i++) {
-                const int row = i * RPI + r0;
-                const IN* e = reinterpret_cast<const IN*>(r + 4 * i);
-                const bool sub = !kv && (kind == 2 || (kind == 3 && kt.seen(j0 + row, t.p1)));
                 uint32_t p[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    p[k] = kv ? h2_pack(to_f32(e[2 * k]), to_f32(e[2 * k + 1]))
-                              : h2_pack(to_f32(e[2 * k]) - (sub ? rf8[2 * k] : 0.0f), to_f32(e[2 * k + 1]) - (sub ? rf8[2 * k + 1] : 0.0f));
-                st_chunk(dst + tile_off(row, cc), p[0], p[1], p[2], p[3]);
-            }
-            if (kind != 3) return;
-#pragma unroll 1
-            for (int i = 0; i < NI; i++) {                                         // its cached tokens, one row after the other
-                const int row = i * RPI + r0, j = j0 + row;
-                if (!kt.seen(j, t.p1) || j >= (kv ? t.ctx : full)) continue;
-                const uint8_t* rec = hcache + int64_t(bt[j / P]) * a.block_stride;
-                const int at = j % P;
-                float y[8];
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const int d = 8 * cc + k;
-                    y[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + at * F::DC, d)), h_load(rec + F::OFF_VS, at),
-                                     h_load(rec + F::OFF_VB, at))
-                              : fmaf(float(code_at<D, BITS>(rec + at * F::DC, d)), h_load(rec + F::OFF_KS, d),
-                                     h_load(rec + F::OFF_KB, d)) - rf8[k];
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t e = r[4 * i + k];                               // two channels
+                    if constexpr (std::is_same_v<IN, __half>) {
+                        p[k] = kv ? e : h2_sub_u(e, h2_pack(-minus[k].x, -minus[k].y));
+                    } else {
+                        float2 y = make_float2(__uint_as_float(e << 16), __uint_as_float(e & 0xFFFF0000u));
+                        if constexpr (!kv) y = __fadd2_rn(y, minus[k]);
+                        p[k] = h2_pack(y.x, y.y);
+                    }
                 }
-                st_chunk(dst + tile_off(row, cc), h2_pack(y[0], y[1]), h2_pack(y[2], y[3]), h2_pack(y[4], y[5]), h2_pack(y[6], y[7]));
+                // (rows RPI apart: the swizzle's upper bits)
+                const uint32_t flip = RPI == 2 ? (i & 3) << 5 : (i & 1) << 6;
+                st_chunk(dst + ((at_r ^ flip) + RPI * 128 * i), p[0], p[1], p[2], p[3]);
             }
         };
         int32_t f = __shfl_sync(0xffffffffu, from, 0), bl = __shfl_sync(0xffffffffu, blk, 0);
