@@ -244,38 +244,46 @@ class Ops:
         [rows, H, D] (either may be None; row and head strides free, e.g. parts of q|k|v rows), row i at positions[i]
         (int32 or int64, contiguous), into q_out and k_out (new tensors, or q and k themselves, or others of their
         shapes).  Returns (q_out, k_out).  Angles are exact to fp32 for every position; one rounding to the dtype."""
-        D, rows = self.D, positions.numel()
-        _need(positions.dtype in (torch.int64, torch.int32) and positions.is_contiguous(),
-              "rope: positions must be contiguous int32 or int64")
-        _need(rotary.head_dim == D and rotary.turns.device == self.device,
-              f"rope: the plan must be one of rotary() for head_dim {D} on {self.device}")
-        args = []
-        outs = []
+        D, rows, dt = self.D, positions.shape[0] if positions.dim() == 1 else -1, self.dtype
+        wide = positions.dtype == torch.int64
+        if rows < 0 or not (wide or positions.dtype == torch.int32) or not positions.is_contiguous():
+            raise ValueError("rope: positions must be a contiguous row of int32 or int64")
+        if rotary.head_dim != D or rotary.turns.device != self.device:
+            raise ValueError(f"rope: the plan must be one of rotary() for head_dim {D} on {self.device}")
+        args, outs = [], []
         for x, y in ((q, q_out), (k, k_out)):
             if x is None:
-                _need(y is None, "rope: an output without its input")
+                if y is not None:
+                    raise ValueError("rope: an output without its input")
                 args += (None, 0, 0, None, 0, 0, 0)
                 outs.append(None)
                 continue
             if y is None:
                 y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            _need(x.dtype == self.dtype and y.dtype == self.dtype, f"rope: rows must be {self.dtype}")
-            _need(x.dim() == 3 and x.shape[0] == rows and x.shape[2] == D and x.shape == y.shape and x.stride(2) == 1
-                  and y.stride(2) == 1, f"rope: rows must be [{rows}, heads, {D}] with contiguous channels, "
-                  "outputs of their inputs' shapes")
-            args += (x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(), y.stride(0), y.stride(1), x.shape[1])
+            xs, ys, shape = x.stride(), y.stride(), x.shape
+            if x.dtype != dt or y.dtype != dt:
+                raise ValueError(f"rope: rows must be {dt}")
+            if len(shape) != 3 or shape[0] != rows or shape[2] != D or shape != y.shape or xs[2] != 1 or ys[2] != 1:
+                raise ValueError(f"rope: rows must be [{rows}, heads, {D}] with contiguous channels, outputs of their inputs' "
+                                 "shapes")
+            args += (x.data_ptr(), xs[0], xs[1], y.data_ptr(), ys[0], ys[1], shape[1])
             outs.append(y)
         self._run("kush_sm100_rope", D, self.cfg.dtype_code, rotary.rotary_dim, int(rotary.interleaved), *args,
-                  positions.data_ptr(), int(positions.dtype == torch.int64), rotary.turns.data_ptr(), rotary.factor, rows)
+                  positions.data_ptr(), int(wide), rotary.turns.data_ptr(), rotary.factor, rows)
         return outs[0], outs[1]
 
     # ---------------------------------------------------------------- decode
     def splits(self, num_seqs: int, num_kv_heads: int, max_full_pages: int, *, window: int | None = None,
                sinks: int = 0) -> int:
         """Split-KV factor for this device (split_factor); under a window, of the pages a query sees."""
-        if window is not None:
-            max_full_pages = min(max_full_pages, -(-window // self.P) + 1 + -(-sinks // self.P))
-        return split_factor(num_seqs, num_kv_heads, max_full_pages, self.sms)
+        if window is None:
+            return split_factor(num_seqs, num_kv_heads, max_full_pages, self.sms)
+        # a windowed unit has few pages, so a second wave of CTAs costs as much as the first: count the CTAs that are resident
+        # at once with this configuration's registers (61 sequences x 4 kv heads of 34 int8 pages: one split 37 us, two 47)
+        wide = self.D == 256 or self.G > 8
+        resident = 4 if self.D == 64 and not wide else 2 if wide else 3 if self.bits == 8 and self.P == 32 else 4
+        pages = min(max_full_pages, -(-window // self.P) + 1 + -(-sinks // self.P))
+        return split_factor(num_seqs, num_kv_heads, pages, self.sms, resident)
 
     def work_size(self, num_seqs: int, num_kv_heads: int, n_splits: int, fused: bool = False) -> int:
         """fp32 elements of the split-KV work buffer: S * Hkv * n_splits * G * (D + 2), the (M, L) pairs first, then
@@ -359,10 +367,11 @@ class Ops:
                        part_ml: int, part_o: int, rotate: bool, order: torch.Tensor | None, fused: bool,
                        window: int | None, sinks: int) -> None:
         S, H = q.shape[0], tail_k.shape[1]
-        _need(window is not None and window >= 1 and sinks >= 0,
-              f"decode: window must be >= 1 and sinks >= 0 (sinks need a window), got {window} and {sinks}")
-        _need(order is None or (order.dtype == torch.int32 and order.numel() == S and order.is_contiguous()),
-              "decode: order must be a contiguous int32 permutation of the sequences")
+        if window is None or window < 1 or sinks < 0:
+            raise ValueError(f"decode: window must be >= 1 and sinks >= 0 (sinks need a window), got {window} and {sinks}")
+        if order is not None:
+            _need(order.dtype == torch.int32 and order.numel() == S and order.is_contiguous(),
+                  "decode: order must be a contiguous int32 permutation of the sequences")
         counters = part_ml + 4 * S * H * n_splits * self.G * (self.D + 2) if fused and n_splits > 1 else None
         self._run("kush_sm100_decode_window", *self._fmt, self.G, q.data_ptr(), out.data_ptr(), *_pool(cache),
                   tail_k.data_ptr(), tail_idx.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
@@ -399,23 +408,28 @@ class Ops:
         position.  n_splits > 1 (chunk_splits()) divides each tile's keys over more blocks and needs `work`
         (chunk_work_size() fp32 elements).  Over a rotated cache, give it fwht() of q, k and v (write() wants the
         latter two as well) and take fwht() of out."""
-        D, rows, S, H = self.D, q.shape[0], seq_lens.numel(), k.shape[1]
-        _need(q.dtype == self.dtype and k.dtype == self.dtype and v.dtype == self.dtype and out.dtype == self.dtype
-              and tail_k.dtype == self.dtype, f"attend_chunk: q, k, v, out and tail_k must be {self.dtype}")
-        _need(q.dim() == 3 and q.shape[1] == H * self.G and q.shape[2] == D and q.stride(1) == D and q.stride(2) == 1,
-              f"attend_chunk: q must be [rows, H * {self.G}, {D}] with head stride {D}")
-        _need(k.shape == (rows, H, D) == tuple(v.shape) and k.stride()[1:] == (D, 1) == v.stride()[1:],
-              f"attend_chunk: k and v must be [{rows}, H, {D}] with head stride {D}")
-        _need(out.shape == q.shape and out.is_contiguous(), "attend_chunk: out must be contiguous, of q's shape")
-        _need(tail_k.dim() == 4 and tuple(tail_k.shape[1:]) == (H, self.P, D) and tail_k.is_contiguous(),
-              f"attend_chunk: tail_k must be contiguous [slots, {H}, {self.P}, {D}]")
-        _need(query_start_loc.dtype == seq_lens.dtype == tail_idx.dtype == block_table.dtype == torch.int32
-              and query_start_loc.is_contiguous() and seq_lens.is_contiguous() and tail_idx.is_contiguous()
-              and query_start_loc.numel() == S + 1 and tail_idx.numel() >= S and block_table.shape[0] >= S
-              and block_table.stride(1) == 1, "attend_chunk: query_start_loc [S + 1], seq_lens and tail_idx [S] must be "
-              "contiguous int32, block_table [S, pages] int32 with contiguous rows")
-        _need((window is None or window >= 1) and sinks >= 0 and (window is not None or sinks == 0),
-              f"attend_chunk: window must be >= 1 and sinks >= 0 (sinks need a window), got {window} and {sinks}")
+        D, G, dt, S = self.D, self.G, self.dtype, seq_lens.shape[0]
+        qs, ks, vs, shape = q.stride(), k.stride(), v.stride(), k.shape
+        if not (q.dtype == k.dtype == v.dtype == out.dtype == tail_k.dtype == dt):
+            raise ValueError(f"attend_chunk: q, k, v, out and tail_k must be {dt}")
+        if len(shape) != 3 or shape[2] != D or v.shape != shape or ks[1:] != (D, 1) or vs[1:] != (D, 1):
+            raise ValueError(f"attend_chunk: k and v must be [rows, H, {D}] with head stride {D}")
+        rows, H = shape[0], shape[1]
+        if tuple(q.shape) != (rows, H * G, D) or qs[1:] != (D, 1):
+            raise ValueError(f"attend_chunk: q must be [{rows}, {H * G}, {D}] with head stride {D}")
+        if out.shape != q.shape or not out.is_contiguous():
+            raise ValueError("attend_chunk: out must be contiguous, of q's shape")
+        if tuple(tail_k.shape[1:]) != (H, self.P, D) or not tail_k.is_contiguous():
+            raise ValueError(f"attend_chunk: tail_k must be contiguous [slots, {H}, {self.P}, {D}]")
+        i32 = torch.int32
+        if (not (query_start_loc.dtype == seq_lens.dtype == tail_idx.dtype == block_table.dtype == i32)
+                or tuple(query_start_loc.shape) != (S + 1,) or tail_idx.shape[0] < S or block_table.shape[0] < S
+                or not query_start_loc.is_contiguous() or not seq_lens.is_contiguous() or not tail_idx.is_contiguous()
+                or block_table.stride(1) != 1):
+            raise ValueError("attend_chunk: query_start_loc [S + 1], seq_lens and tail_idx [S] must be contiguous int32, "
+                             "block_table [S, pages] int32 with contiguous rows")
+        if (window is None and sinks) or sinks < 0 or (window is not None and window < 1):
+            raise ValueError(f"attend_chunk: window must be >= 1 and sinks >= 0 (sinks need a window), got {window} and {sinks}")
         part_o = part_ml = None
         if n_splits > 1:
             need = self.chunk_work_size(rows, H, n_splits)
@@ -423,8 +437,8 @@ class Ops:
                   f"attend_chunk: n_splits={n_splits} needs a contiguous fp32 work buffer of >= {need} elements")
             part_o = work.data_ptr()
             part_ml = part_o + 4 * rows * H * n_splits * self.G * D
-        self._run("kush_sm100_attend_chunk", *self._fmt, self.G, q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(),
-                  k.stride(0), v.stride(0), out.data_ptr(), query_start_loc.data_ptr(), seq_lens.data_ptr(),
+        self._run("kush_sm100_attend_chunk", *self._fmt, G, q.data_ptr(), qs[0], k.data_ptr(), v.data_ptr(),
+                  ks[0], vs[0], out.data_ptr(), query_start_loc.data_ptr(), seq_lens.data_ptr(),
                   tail_idx.data_ptr(), *_pool(cache), tail_k.data_ptr(), *_table(block_table), H, float(scale),
                   min(window, _I32_MAX) if window is not None else 0, min(sinks, _I32_MAX), n_splits, part_ml, part_o, rows,
                   S)

@@ -433,7 +433,10 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
     const VisiblePages vis = WIN ? visible_pages(int32_t(n), window, sinks, P) : VisiblePages{};
     const SplitRange sr = WIN ? split_range_window(seq_lens, int(gridDim.x), vis, z, n_splits, window, sinks, P)
                               : split_range(seq_lens, int(gridDim.x), s, z, n_splits, P);
-    auto page_at = [&](int64_t i) -> int64_t { return WIN ? vis.page(i) : i; };       // logical page of range index i
+    const int32_t gap = WIN ? vis.b - vis.a : 0;
+    auto page_at = [&](int64_t i) -> int64_t {                                        // logical page of range index i
+        return WIN ? i + (i >= vis.a ? gap : 0) : i;
+    };
     if (!sr.active) {                                                   // no pages here: an empty partial
         for (int hd = threadIdx.x; hd < G; hd += NW * WARP) {
             const int64_t pb = ((int64_t(s) * H + h) * n_splits + z) * G + hd;
@@ -547,6 +550,14 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
         }
     bool ok = true;
     int fail_at = npw;
+    // WIN: the page of this warp that a border of the visible tokens cuts (range index a - 1 or a, of which a warp has at
+    // most one), or -1
+    int cut_at = -1;
+    if constexpr (WIN) {
+        const int64_t c0 = vis.a - 1 - mine0, c1 = vis.a - mine0;
+        if (c0 >= 0 && c0 % NW == 0 && vis.ns < vis.a * P) cut_at = int(c0 / NW);
+        if (c1 >= 0 && c1 % NW == 0 && vis.lo > vis.b * P) cut_at = int(c1 / NW);
+    }
 
 #pragma unroll 1
     for (int i = 0; i < npw; i++) {
@@ -560,11 +571,21 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
         const uint8_t* scl = C::SPLIT ? wscl + slot * C::SCALES : codes + C::CODES;   // ks, kb, vs, vb
         // one 16-token tile at a time (P = 32 pages have two): QK, online softmax, PV.  The softmax is tile-granular,
         // which keeps the register footprint of both page sizes the same.
-        const int64_t tok0 = WIN ? page_at(mine0 + int64_t(i) * NW) * P : 0;    // the page's first token
+        // (WIN: a page that a border cuts takes its own copy of the code, so that the others' keeps the plain kernel's)
+        auto tiles = [&](auto cut) {
+        constexpr bool CUT = decltype(cut)::value != 0;
+        // a border cuts this page: its first token, and the borders (worked out again: they would cost the loop registers)
+        int32_t cut0 = 0, cut_ns = 0, cut_lo = 0;
+        if constexpr (CUT) {
+            const VisiblePages v = visible_pages(seq_lens[s], window, sinks, P);
+            cut0 = int32_t(v.page(mine0 + int64_t(i) * NW)) * P;
+            cut_ns = v.ns;
+            cut_lo = v.lo;
+        }
 #pragma unroll
         for (int mtt = 0; mtt < MTT; mtt++) {
-            if constexpr (WIN) {
-                if (tok0 + mtt * 16 >= vis.ns && tok0 + mtt * 16 + 16 <= vis.lo) continue;    // no visible token
+            if constexpr (CUT) {
+                if (cut0 + mtt * 16 >= cut_ns && cut0 + mtt * 16 + 16 <= cut_lo) continue;    // no visible token
             }
             float sc[NT][4];
             {
@@ -601,16 +622,13 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
                     sc[nt][3] = a23.y;
                 }
             }
-            if constexpr (WIN) {
-                const int64_t t0 = tok0 + mtt * 16;
-                if (t0 < vis.lo && t0 + 16 > vis.ns) {                     // a border cuts this tile
+            if constexpr (CUT) {
 #pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const int64_t t = t0 + g + 8 * r;
-                        if (t >= vis.ns && t < vis.lo) {
+                for (int r = 0; r < 2; r++) {
+                    const int32_t t = cut0 + mtt * 16 + g + 8 * r;
+                    if (t >= cut_ns && t < cut_lo) {
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) sc[nt][2 * r] = sc[nt][2 * r + 1] = -INFINITY;
-                        }
+                        for (int nt = 0; nt < NT; nt++) sc[nt][2 * r] = sc[nt][2 * r + 1] = -INFINITY;
                     }
                 }
             }
@@ -680,6 +698,13 @@ __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB))
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
                     mma16816(o[mt][nt], va[mt][0], va[mt][1], va[mt][2], va[mt][3], pb[nt][0], pb[nt][1]);
+        }
+        };
+        if constexpr (WIN) {
+            if (i == cut_at) tiles(IC<1>{});
+            else tiles(IC<0>{});
+        } else {
+            tiles(IC<0>{});
         }
         __syncwarp();
         // refill this slot with page i + NS
