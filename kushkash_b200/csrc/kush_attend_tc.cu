@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 wait_ld(x);
                 float mx = piece(0, x, y, top(x), IC<0>{});
                 mx = piece(1, y, x, mx, IC<0>{});
+                pass_on();                                                         // (half of it left: the exponentials of both overlap)
                 mx = piece(2, x, y, mx, IC<0>{});
-                pass_on();
                 piece(3, y, x, mx, IC<1>{});
                 wait_st();
             }
