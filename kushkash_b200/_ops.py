@@ -117,6 +117,12 @@ class Ops:
                 rc = fn(*args, _cuda.raw_stream(self.dev))
         _cuda.check(rc, entry)
 
+    def _here(self, what: str, *tensors: torch.Tensor) -> None:
+        """Refuse tensors of another device: their addresses would fault in a kernel."""
+        for t in tensors:
+            if t.get_device() != self.dev:
+                raise ValueError(f"{what}: every tensor must be on {self.device}, got one on {t.device}")
+
     # ---------------------------------------------------------------- quantize-on-write
     def append(self, k: torch.Tensor, v: torch.Tensor, seq_lens: torch.Tensor, tail_idx: torch.Tensor,
                cache: torch.Tensor, block_table: torch.Tensor, tail_k: torch.Tensor, pos_offset: int, advance: bool,
@@ -248,6 +254,7 @@ class Ops:
         wide = positions.dtype == torch.int64
         if rows < 0 or not (wide or positions.dtype == torch.int32) or not positions.is_contiguous():
             raise ValueError("rope: positions must be a contiguous row of int32 or int64")
+        self._here("rope", positions, *(t for t in (q, k, q_out, k_out) if t is not None))
         if rotary.head_dim != D or rotary.turns.device != self.device:
             raise ValueError(f"rope: the plan must be one of rotary() for head_dim {D} on {self.device}")
         args, outs = [], []
@@ -367,6 +374,7 @@ class Ops:
                        part_ml: int, part_o: int, rotate: bool, order: torch.Tensor | None, fused: bool,
                        window: int | None, sinks: int) -> None:
         S, H = q.shape[0], tail_k.shape[1]
+        self._here("decode", q, out, cache, block_table, seq_lens, tail_idx, tail_k)
         if window is None or window < 1 or sinks < 0:
             raise ValueError(f"decode: window must be >= 1 and sinks >= 0 (sinks need a window), got {window} and {sinks}")
         if order is not None:
@@ -410,6 +418,7 @@ class Ops:
         latter two as well) and take fwht() of out."""
         D, G, dt, S = self.D, self.G, self.dtype, seq_lens.shape[0]
         qs, ks, vs, shape = q.stride(), k.stride(), v.stride(), k.shape
+        self._here("attend_chunk", q, k, v, out, query_start_loc, seq_lens, tail_idx, cache, block_table, tail_k)
         if not (q.dtype == k.dtype == v.dtype == out.dtype == tail_k.dtype == dt):
             raise ValueError(f"attend_chunk: q, k, v, out and tail_k must be {dt}")
         if len(shape) != 3 or shape[2] != D or v.shape != shape or ks[1:] != (D, 1) or vs[1:] != (D, 1):
@@ -433,8 +442,8 @@ class Ops:
         part_o = part_ml = None
         if n_splits > 1:
             need = self.chunk_work_size(rows, H, n_splits)
-            _need(work is not None and work.dtype == torch.float32 and work.is_contiguous() and work.numel() >= need,
-                  f"attend_chunk: n_splits={n_splits} needs a contiguous fp32 work buffer of >= {need} elements")
+            _need(work is not None and work.dtype == torch.float32 and work.is_contiguous() and work.numel() >= need
+                  and work.get_device() == self.dev, f"attend_chunk: n_splits={n_splits} needs a contiguous fp32 work buffer of >= {need} elements")
             part_o = work.data_ptr()
             part_ml = part_o + 4 * rows * H * n_splits * self.G * D
         self._run("kush_sm100_attend_chunk", *self._fmt, G, q.data_ptr(), qs[0], k.data_ptr(), v.data_ptr(),

@@ -1,7 +1,8 @@
-// Async-copy and bit-manipulation helpers shared by the decode and write kernels: shared-memory addresses, PRMT,
+// Async-copy, bit-manipulation and half-precision helpers shared by the decode, attention and write kernels: shared-memory addresses, PRMT,
 // mbarrier init / bounded wait, and the fence that publishes mbarrier initialisation.  No multicast anywhere.
 #pragma once
 
+#include <cuda_fp16.h>
 #include <stdint.h>
 
 namespace kush {
@@ -36,4 +37,29 @@ __device__ __forceinline__ bool mbar_wait_u32(uint32_t bar, uint32_t parity) {
 
 __device__ __forceinline__ void fence_mbar_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 
+// (a & b) ^ c in one LOP3
+__device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 }  // namespace kush

@@ -121,9 +121,10 @@ extern "C" int kush_sm100_attend_chunk(int32_t head_dim, int32_t bits, int32_t p
     a.H = hkv;
     a.G = group;
     a.S = n_seqs;
+    a.n_rows = int32_t(n_rows);
     a.sm_log2 = scale * 1.4426950408889634f;
-    a.window = window;
-    a.sinks = sinks;
+    a.window = window < KUSH_NO_POSITION ? window : KUSH_NO_POSITION;     // (differences of positions stay in 32 bits)
+    a.sinks = sinks < KUSH_NO_POSITION ? sinks : KUSH_NO_POSITION;
     a.n_splits = n_splits;
     a.part_ml = part_ml;
     a.part_o = part_o;

@@ -10,6 +10,8 @@
 
 namespace kush {
 
+constexpr int32_t KUSH_NO_POSITION = 1 << 30;      // above every position
+
 struct AttendArgs {
     const void* q;
     void* out;
@@ -22,6 +24,7 @@ struct AttendArgs {
     const int32_t *tail_idx, *block_table, *seq_lens, *qsl;      // qsl null in decode
     int64_t max_pages;
     int32_t H, G, S;
+    int32_t n_rows;                  // rows of q, k_new and v_new (query_start_loc is not believed beyond them)
     float sm_log2;                   // scale * log2(e)
     int32_t window, sinks;           // window 0: none
     int32_t n_splits;
@@ -55,7 +58,7 @@ __device__ __forceinline__ bool row_tile(const AttendArgs& a, int x, int TM, Row
     int base = 0;
     for (int i0 = 0; i0 < a.S; i0 += WARP) {
         const int i = i0 + lane;
-        const int n = i < a.S ? max(0, a.qsl[i + 1] - a.qsl[i]) : 0;
+        const int n = i < a.S ? max(0, min(a.qsl[i + 1], a.n_rows) - max(0, a.qsl[i])) : 0;
         const int cnt = int((int64_t(n) * a.G + TM - 1) / TM);
         int sum = cnt;
 #pragma unroll
@@ -70,7 +73,7 @@ __device__ __forceinline__ bool row_tile(const AttendArgs& a, int x, int TM, Row
             t.n_new = __shfl_sync(0xffffffffu, n, l);
             t.r0 = (x - base - __shfl_sync(0xffffffffu, sum - cnt, l)) * TM;
             t.nr = int(min(int64_t(TM), int64_t(t.n_new) * a.G - t.r0));
-            t.q0 = a.qsl[t.s];
+            t.q0 = max(0, a.qsl[t.s]);
             t.ctx = max(0, a.seq_lens[t.s] - t.n_new);
             t.p0 = t.ctx + t.r0 / a.G;
             t.p1 = t.ctx + (t.r0 + t.nr - 1) / a.G;

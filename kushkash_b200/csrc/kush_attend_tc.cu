@@ -10,13 +10,33 @@
 // converted; fp16), one thread of warps 14 and 15 issues the products of slots 0 and 1:
 //   S[128 x 128] = Q K'^T   (both from shared memory, K-major, 128-byte swizzle), fp32 in TMEM
 //   O[128 x D]  += P V      (P fp16 in TMEM over the first half of S's columns, V from shared memory, N-major)
+// (softmax warps that have no rows bring keys and values too: 20 rows of drafted tokens leave six of them.)
 // K' = c ks + (kb - ref), fp16, ref = the key bias of the first finished page the block sees: the same shift of every
 // score of a row, which the softmax drops; large channel offsets are gone before the rounding to fp16.  q and the new
 // rows enter as fp16 too (exact for bf16 within fp16's range, which the cache's own fp16 scales have as well).  Scores,
 // maxima, sums and outputs stay fp32; the weights p = 2^(s - m) <= 2^8 are rounded once to fp16.  The maximum moves
 // lazily: O is rescaled only when a score passes the maximum in use by 2^8.
 //
+// What bounds it.  A pair of 128-row tiles and a key tile are 32 products of 64 cycles (2048 cycles of tensor cores), 32768
+// exponentials at 16 a cycle (2048 cycles) and 32768 dequantized values, all on four schedulers: none of the three alone,
+// their sum of issue slots and the chain product -> softmax -> product do.  One wave of blocks (1152 rows of 4 q heads on 8
+// kv heads over 30001 int4 tokens, bf16) takes 616 us = 936 TFLOP/s, 57% of the measured bf16 GEMM rate; with the
+// conversions left out 556, the softmax's arithmetic left out 497, both 449.  8192 new rows without history: 628 us = 876.
+// What the design rests on, measured on that wave or on a 2048-row chunk:
+//   two slots                    one issuing warp per slot: with one for both, its waits and issue left the tensor cores idle
+//                                (4200 cycles a tile for itself); operands in uniform registers (elect.sync, shuffled
+//                                values): a product's issue fell from 80 to 20 cycles
+//   turns of the two softmaxes   847 -> 927 TFLOP/s, passed on at half a softmax 936 (at the end 893)
+//   units loaded a unit ahead    keys under the values' conversion and the other way round: 824 -> 894 TFLOP/s; a ring of
+//   into registers               bulk copies in shared memory instead cost the producers more instructions than it saved
+//   one pass over S              32 columns at a time; masked scores are rewritten in TMEM first (rolled loops: the code of
+//                                all roles has to stay in the instruction caches; unrolled, 28% of the stalls were fetches)
+//   20 warps, registers moved    ten producing warps of 88 registers by setmaxnreg: spills, 892 TFLOP/s; not kept
+// Short calls (20 rows a sequence) are bound by that chain: 64 sequences x 5 rows over 4000-8192 tokens 361 us.
+//
 // Waits are bounded (2 s): on a timeout the block raises the error flag, writes NaN and returns.
+#include <atomic>
+
 #include "kush_async.cuh"
 #include "kush_attend.cuh"
 
@@ -104,31 +124,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t h2_pack(float lo, float hi) {
-    __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t h2_fma_u(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t h2_sub_u(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t and_xor_u(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-
 // byte offset of (row, 8-channel chunk) in a tile of swizzled blocks
 __device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
     return uint32_t((chunk >> 3) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
@@ -146,18 +141,18 @@ __device__ __forceinline__ void codes_of(const uint32_t (&w)[BITS / 2], uint32_t
         for (int i = 0; i < 2; i++) {
             const uint32_t x = prmt(w[i], 0, 0x3120);             // bytes b0 b2 b1 b3
             const uint32_t y = x >> 8;                             // b2 b1 b3
-            lo[2 * i] = h2_sub_u(and_xor_u(x, 0x000F000Fu, 0x64086408u), 0x64086408u);
-            lo[2 * i + 1] = h2_sub_u(and_xor_u(y, 0x000F000Fu, 0x64086408u), 0x64086408u);
-            hi[2 * i] = h2_fma_u(and_xor_u(x, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u);
-            hi[2 * i + 1] = h2_fma_u(and_xor_u(y, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u);
+            lo[2 * i] = h2_sub(and_xor(x, 0x000F000Fu, 0x64086408u), 0x64086408u);
+            lo[2 * i + 1] = h2_sub(and_xor(y, 0x000F000Fu, 0x64086408u), 0x64086408u);
+            hi[2 * i] = h2_fma(and_xor(x, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u);
+            hi[2 * i + 1] = h2_fma(and_xor(y, 0x00F000F0u, 0x64806480u), 0x2C002C00u, 0xD480D480u);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t u = w[i] ^ 0x80808080u;                 // signed code -> c + 128
             uint32_t(&o)[4] = i < 2 ? lo : hi;
-            o[2 * (i & 1)] = h2_sub_u(prmt(u, 0x64646464u, 0x5140), 0x64806480u);
-            o[2 * (i & 1) + 1] = h2_sub_u(prmt(u, 0x64646464u, 0x7342), 0x64806480u);
+            o[2 * (i & 1)] = h2_sub(prmt(u, 0x64646464u, 0x5140), 0x64806480u);
+            o[2 * (i & 1) + 1] = h2_sub(prmt(u, 0x64646464u, 0x7342), 0x64806480u);
         }
     }
 }
@@ -302,7 +297,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             const IN* e = reinterpret_cast<const IN*>(&raw);
             uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) w[j] = h2_pack(sign * to_f32(e[2 * j]), sign * to_f32(e[2 * j + 1]));
+            for (int j = 0; j < 4; j++) w[j] = pack_h2(sign * to_f32(e[2 * j]), sign * to_f32(e[2 * j + 1]));
             st_chunk(base + M::Q + (r >> 7) * M::TILE + tile_off(r & 127, c), w[0], w[1], w[2], w[3]);
         }
     }
@@ -382,7 +377,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 // weights along.
                 auto move_max = [&](int c, float mx) {
                     const bool up = mx > m + TC_TAU;
-                    const float corr = up ? ex2(m - mx) : 1.0f;                    // first scores: 2^-inf = 0
+                    const float corr = up ? fast_exp2(m - mx) : 1.0f;                    // first scores: 2^-inf = 0
                     if (up) m = mx;
                     la = __fmul2_rn(la, make_float2(corr, corr));
                     lb = __fmul2_rn(lb, make_float2(corr, corr));
@@ -434,7 +429,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                         x[i + 1] = __float_as_uint(d.y);
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; i++) x[i] = __float_as_uint(ex2(__uint_as_float(x[i])));
+                    for (int i = 0; i < 32; i++) x[i] = __float_as_uint(fast_exp2(__uint_as_float(x[i])));
                     float next = 0.0f;
                     if constexpr (!decltype(last)::value) {
                         wait_ld(y);
@@ -446,7 +441,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                         const float2 e = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
                         if (i & 1) lb = __fadd2_rn(lb, e);
                         else la = __fadd2_rn(la, e);
-                        p[i] = h2_pack(e.x, e.y);
+                        p[i] = pack_h2(e.x, e.y);
                     }
                     tmem_st16(s_at + 16 * c, p);
                     return next;
@@ -500,8 +495,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             if (!paired) {
                 mo = xm[row];
                 const float mn = fmaxf(m, mo);
-                f0 = m == -INFINITY ? 0.0f : ex2(m - mn);
-                f1 = mo == -INFINITY ? 0.0f : ex2(mo - mn);
+                f0 = m == -INFINITY ? 0.0f : fast_exp2(m - mn);
+                f1 = mo == -INFINITY ? 0.0f : fast_exp2(mo - mn);
                 l = l * f0 + (f1 > 0.0f ? xm[128 + row] * f1 : 0.0f);
                 m = mn;
             }
@@ -592,8 +587,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         uint32_t rf[8];                                                            // the reference of the lane's channels
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            rf[i] = h2_pack(ref[8 * c_a + 2 * i], ref[8 * c_a + 2 * i + 1]);
-            rf[4 + i] = h2_pack(ref[8 * c_b + 2 * i], ref[8 * c_b + 2 * i + 1]);
+            rf[i] = pack_h2(ref[8 * c_a + 2 * i], ref[8 * c_a + 2 * i + 1]);
+            rf[4 + i] = pack_h2(ref[8 * c_b + 2 * i], ref[8 * c_b + 2 * i + 1]);
         }
         // new rows: chunk cc of rows r0, r0 + RPI, ...
         constexpr int RPI = WARP / CH, NI = 16 / RPI;
@@ -666,7 +661,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                         for (int k = 0; k < 8; k++) y[k] -= ref[8 * cc + k];
                     }
                 }
-                st_chunk(dst + tile_off(row, cc), h2_pack(y[0], y[1]), h2_pack(y[2], y[3]), h2_pack(y[4], y[5]), h2_pack(y[6], y[7]));
+                st_chunk(dst + tile_off(row, cc), pack_h2(y[0], y[1]), pack_h2(y[2], y[3]), pack_h2(y[4], y[5]), pack_h2(y[6], y[7]));
             }
         };
         auto convert = [&](auto kvc, int32_t f, uint32_t (&r)[32], uint32_t dst) {
@@ -675,7 +670,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             if (kind == 1) {
                 if constexpr (!kv) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) r[24 + i] = h2_sub_u(r[24 + i], rf[i]);
+                    for (int i = 0; i < 8; i++) r[24 + i] = h2_sub(r[24 + i], rf[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < U::RPL; i++) {
@@ -688,14 +683,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                         const uint32_t vb = __shfl_sync(0xffffffffu, r[16], 16 + rg + U::RG * i) * 0x10001u;
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            lo[j] = h2_fma_u(lo[j], vs, vb);
-                            hi[j] = h2_fma_u(hi[j], vs, vb);
+                            lo[j] = h2_fma(lo[j], vs, vb);
+                            hi[j] = h2_fma(hi[j], vs, vb);
                         }
                     } else {
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            lo[j] = h2_fma_u(lo[j], r[16 + j], r[24 + j]);
-                            hi[j] = h2_fma_u(hi[j], r[20 + j], r[28 + j]);
+                            lo[j] = h2_fma(lo[j], r[16 + j], r[24 + j]);
+                            hi[j] = h2_fma(hi[j], r[20 + j], r[28 + j]);
                         }
                     }
                     const uint32_t flip = U::RG == 4 && (i & 1) ? 64 : 0;          // rows 4 apart: the swizzle's bit 2
@@ -717,11 +712,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 for (int k = 0; k < 4; k++) {
                     const uint32_t e = r[4 * i + k];                               // two channels
                     if constexpr (std::is_same_v<IN, __half>) {
-                        p[k] = kv ? e : h2_sub_u(e, h2_pack(-minus[k].x, -minus[k].y));
+                        p[k] = kv ? e : h2_sub(e, pack_h2(-minus[k].x, -minus[k].y));
                     } else {
                         float2 y = make_float2(__uint_as_float(e << 16), __uint_as_float(e & 0xFFFF0000u));
                         if constexpr (!kv) y = __fadd2_rn(y, minus[k]);
-                        p[k] = h2_pack(y.x, y.y);
+                        p[k] = pack_h2(y.x, y.y);
                     }
                 }
                 // (rows RPI apart: the swizzle's upper bits)
@@ -859,8 +854,14 @@ int launch_attend_tc(int D, int bits, int P, int dtype, const AttendArgs& a, int
         } else {
             auto kern = attend_tc_kernel<Dc.value, Bc.value, Pc.value, IN>;
             constexpr int smem = TcSmem<Dc.value>::BYTES;
-            const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-            if (e != cudaSuccess) return set_error(KUSH_ERR_CUDA, "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+            static std::atomic<unsigned long long> attr_set{0};                    // one bit per device: the attribute is per device
+            int dev = 0;
+            cudaGetDevice(&dev);
+            if (!(attr_set.load() >> (dev & 63) & 1ull)) {
+                const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                if (e != cudaSuccess) return set_error(KUSH_ERR_CUDA, "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+                attr_set |= 1ull << (dev & 63);
+            }
             launch_pdl(kern, dim3(unsigned(tiles), a.H, a.n_splits), dim3(TC_THREADS), size_t(smem), stream, a);
             return check_launch("attention (tensor cores)");
         }

@@ -188,5 +188,6 @@ extern "C" int kush_sm100_decode_window(int32_t head_dim, int32_t bits, int32_t 
         return set_error(KUSH_ERR_ARG, "kush_sm100_decode_window: window %d must be >= 1, sinks %d >= 0", window, sinks);
     return decode_any(head_dim, bits, page, dtype, group, q, out, cache, block_stride, head_stride, tail_k, tail_idx,
                       block_table, seq_lens, max_pages, hkv, scale, n_splits, part_ml, part_o, n_seqs,
-                      (flags & KUSH_DECODE_ROTATE) ? 1 : 0, order, stream, counters, window, sinks);
+                      (flags & KUSH_DECODE_ROTATE) ? 1 : 0, order, stream, counters,
+                      window < KUSH_NO_POSITION ? window : KUSH_NO_POSITION, sinks < KUSH_NO_POSITION ? sinks : KUSH_NO_POSITION);
 }

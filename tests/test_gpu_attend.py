@@ -194,6 +194,56 @@ def test_chunk_graph_and_stream():
     assert torch.equal(out[:47], step.run(n_splits=3)) and (out[47:] == 7.0).all()
 
 
+@pytest.mark.parametrize("D,bits,G,dtype,P,window,sinks", [(128, 8, 4, torch.float16, 16, 300, 16), (128, 4, 4, torch.bfloat16, 32, None, 0),
+                                                            (64, 8, 1, torch.bfloat16, 16, 129, 5)])
+def test_chunk_many_passes_agree(D, bits, G, dtype, P, window, sinks):
+    """Passes in a row without a wait between them, on two steps in turn: the same bits every time, no wait given up."""
+    from kushkash_b200 import _cuda
+    ops = ops_of(D, bits, G, dtype, P)
+    c = Cache(ops, [1300, 0, 517, 2000], 4, seed=bits)
+    if window is not None:
+        c.hide(c.lens, window, sinks)
+    steps = [Step(c, [300, 130, 5, 77], seed=s, spare=0) for s in (1, 2)]
+    want = [s.run(window, sinks) for s in steps]
+    outs = []
+    for i in range(200):
+        s = steps[i % 2]
+        outs.append(torch.empty_like(want[0]))
+        ops.attend_chunk(s.q, s.k, s.v, outs[-1], s.qsl, s.seq_lens, c.tail_idx, c.pool, c.block_table, c.tail_k, D ** -0.5,
+                         window=window, sinks=sinks)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(outs))
+    assert _cuda.device_error() == 0
+
+
+def test_chunk_in_place_and_negative_scale():
+    """out may be q itself; a negative scale attends to the smallest products."""
+    ops = ops_of(128, 4, 4, torch.bfloat16, 16)
+    c = Cache(ops, [200], 2, seed=12)
+    s = Step(c, [150], seed=3, spare=0)
+    args = (s.qsl, s.seq_lens, c.tail_idx, c.pool, c.block_table, c.tail_k)
+    q, want, neg = s.q.contiguous(), torch.empty(150, 8, 128, dtype=torch.bfloat16, device="cuda"), None
+    ops.attend_chunk(q, s.k, s.v, want, *args, 0.07)
+    neg = torch.empty_like(want)
+    ops.attend_chunk(-q, s.k, s.v, neg, *args, -0.07)
+    ops.attend_chunk(q, s.k, s.v, q, *args, 0.07)
+    torch.cuda.synchronize()
+    assert torch.equal(neg, want) and torch.equal(q, want)
+
+
+def test_chunk_row_bounds_beyond_the_rows():
+    """A query_start_loc that runs past the rows: only rows that are there are read and written."""
+    ops = ops_of(128, 4, 4, torch.bfloat16, 16)
+    c = Cache(ops, [64, 32], 1, seed=2)
+    s = Step(c, [8, 12], seed=4, spare=0)
+    want = s.run()
+    out = torch.full((20, 4, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.attend_chunk(s.q, s.k, s.v, out, torch.tensor([0, 8, 500], dtype=torch.int32, device="cuda"), s.seq_lens, c.tail_idx,
+                     c.pool, c.block_table, c.tail_k, 128 ** -0.5)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
 def test_chunk_empty_step():
     ops = ops_of(128, 4, 4, torch.bfloat16, 16)
     c = Cache(ops, [20, 0], 1, seed=8)
@@ -214,6 +264,7 @@ def test_chunk_refusals():
     for bad in (dict(q=s.q.float()), dict(k=s.k[:3]), dict(v=s.v[:, :, :64]), dict(out=out[:, :2]), dict(window=0), dict(sinks=1),
                 dict(window=3, sinks=-1), dict(n_splits=2), dict(n_splits=2, work=torch.empty(10, device="cuda")),
                 dict(query_start_loc=s.qsl.long()), dict(seq_lens=s.seq_lens.repeat(2)), dict(tail_k=c.tail_k[:, :, :8]),
-                dict(q=odd), dict(n_splits=0)):
+                dict(q=odd), dict(n_splits=0), dict(q=s.q.cpu()), dict(block_table=c.block_table.cpu()),
+                dict(n_splits=2, work=torch.empty(1 << 16))):
         with pytest.raises(ValueError):
             ops.attend_chunk(**{**good, **bad})

@@ -124,7 +124,7 @@ def test_rope_refusals():
     other = ops_of(64, torch.bfloat16).rotary()
     for args in ((q.float(), None, pos, plan), (q, None, pos[:3], plan), (q, None, pos.float(), plan), (q[..., :64], None, pos, plan),
                  (q, None, pos, other), (None, None, pos, plan, q), (q, None, pos, plan, q[:, :1]),
-                 (q.transpose(1, 2), None, pos, plan), (q, None, pos.repeat(2)[::2], plan)):
+                 (q.cpu(), None, pos, plan), (q, None, pos.cpu(), plan), (q, q.cpu(), pos, plan), (q.transpose(1, 2), None, pos, plan), (q, None, pos.repeat(2)[::2], plan)):
         with pytest.raises(ValueError):
             ops.rope(*args)
     for bad in (3, 0, 130):

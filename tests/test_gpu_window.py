@@ -129,3 +129,5 @@ def test_window_refusals():
             ops.decode(q, torch.empty_like(q), c.pool, c.block_table, c.seq_lens, c.tail_idx, c.tail_k, 0.1, **kw)
     with pytest.raises(ValueError):
         ops.decode(q, torch.empty_like(q), c.pool, c.block_table, c.seq_lens, c.tail_idx, c.tail_k, 0.1, 2, None, window=4)
+    with pytest.raises(ValueError):
+        ops.decode(q, torch.empty_like(q), c.pool, c.block_table, c.seq_lens.cpu(), c.tail_idx, c.tail_k, 0.1, window=4)
