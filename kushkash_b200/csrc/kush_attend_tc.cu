@@ -31,6 +31,8 @@
 //   into registers               bulk copies in shared memory instead cost the producers more instructions than it saved
 //   one pass over S              32 columns at a time; masked scores are rewritten in TMEM first (rolled loops: the code of
 //                                all roles has to stay in the instruction caches; unrolled, 28% of the stalls were fetches)
+//   exponentials on the FMA pipe  4, 8, 12, 16 of 32 by a polynomial: 906, 886, 865, 840 TFLOP/s; not kept (issue, not the
+//                                exponential unit, is short)
 //   20 warps, registers moved    ten producing warps of 88 registers by setmaxnreg: spills, 892 TFLOP/s; not kept
 // Short calls (20 rows a sequence) are bound by that chain: 64 sequences x 5 rows over 4000-8192 tokens 361 us.
 //
