@@ -393,6 +393,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                         for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
                         tmem_st32(o_at + 32 * e, x);
                     }
+                    wait_st();                                                     // (read back below)
 #pragma unroll 1
                     for (int e = 0; e < c; e++) {                                  // P's pieces before this one
                         uint32_t x[32], p[16];

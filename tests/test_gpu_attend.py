@@ -194,6 +194,26 @@ def test_chunk_graph_and_stream():
     assert torch.equal(out[:47], step.run(n_splits=3)) and (out[47:] == 7.0).all()
 
 
+@pytest.mark.parametrize("order", ["rising", "falling", "both"])
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("ctx", [0, 260])
+def test_chunk_scores_that_move_the_maximum(order, D, dtype, ctx):
+    """Scores that rise by about one per token, so that every 32 columns pass the running maximum by more than its slack,
+    fall, or rise for some rows and fall for others."""
+    ops = ops_of(D, 8, 2, dtype, 16)
+    c = Cache(ops, [ctx], 1, seed=1)
+    n = 300
+    step = Step(c, [n], seed=2, spare=0)
+    u = torch.sign(torch.randn(D, generator=torch.Generator().manual_seed(3))).cuda()
+    ramp = torch.arange(n, device="cuda", dtype=torch.float32) * (8.0 / D)          # score / position: 8 D^-1/2, ~1 per token
+    step.k[:, 0] = (u * ramp[:, None]).to(dtype)
+    sign = {"rising": torch.ones(n), "falling": -torch.ones(n), "both": 1.0 - 2.0 * (torch.arange(n) % 2)}[order].cuda()
+    step.q[:] = (u * sign[:, None, None]).to(dtype)
+    want, bound = step.reference(None, 0)
+    for n_splits in (1, 2):
+        check(step.run(None, 0, n_splits), want, bound, dtype, f"{order} scores, ctx {ctx}, splits {n_splits}")
+
+
 @pytest.mark.parametrize("D,bits,G,dtype,P,window,sinks", [(128, 8, 4, torch.float16, 16, 300, 16), (128, 4, 4, torch.bfloat16, 32, None, 0),
                                                             (64, 8, 1, torch.bfloat16, 16, 129, 5)])
 def test_chunk_many_passes_agree(D, bits, G, dtype, P, window, sinks):
