@@ -169,7 +169,8 @@ int kush_sm100_decode_fused_combine(int32_t head_dim, int32_t bits, int32_t page
 /* kush_sm100_decode_fused_combine under a sliding window with sink tokens: the query of sequence s, at position
  * seq_lens[s] - 1, sees the last `window` tokens (itself among them) and the first `sinks` ones; window >= 1, sinks >= 0.
  * Pages without a visible token are not read, nor their block-table entries (the caller may have given them back).
- * counters: as there, or NULL to merge n_splits > 1 with kush_sm100_combine(_rotated).  Splits divide the visible pages.
+ * out is complete: counters as there, or NULL for n_splits > 1 to be merged by a second launch of this call.  Splits
+ * divide the visible pages.
  * flags and order as kush_sm100_decode_ex (the rotated form takes the order here).  No counterpart in the reference. */
 int kush_sm100_decode_window(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group, const void *q,
                              void *out, const void *cache, int64_t block_stride, int64_t head_stride,

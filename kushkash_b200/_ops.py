@@ -110,7 +110,7 @@ class Ops:
     def _run(self, entry: str, *args) -> None:
         """Call one C entry point with torch's current stream of this device appended; raise on a failed status."""
         fn = getattr(self.lib, entry)
-        if torch.cuda.current_device() == self.dev:
+        if torch._C._cuda_getDevice() == self.dev:           # (CUDA is up since __init__)
             rc = fn(*args, _cuda.raw_stream(self.dev))
         else:
             with torch.cuda.device(self.dev):
@@ -386,9 +386,6 @@ class Ops:
                   block_table.stride(0), H, float(scale), n_splits, part_ml or None, part_o or None, counters, S,
                   1 if rotate else 0, order.data_ptr() if order is not None else None, min(window, _I32_MAX),
                   min(sinks, _I32_MAX))
-        if n_splits > 1 and counters is None:
-            entry = "kush_sm100_combine_rotated" if rotate else "kush_sm100_combine"
-            self._run(entry, self.D, self.cfg.dtype_code, self.G, out.data_ptr(), part_ml, part_o, n_splits, H, S)
 
     # ---------------------------------------------------------------- chunk attention
     def chunk_splits(self, num_rows: int, num_seqs: int, num_kv_heads: int, max_len: int, *, window: int | None = None,

@@ -186,8 +186,12 @@ extern "C" int kush_sm100_decode_window(int32_t head_dim, int32_t bits, int32_t 
     if (flags & ~KUSH_DECODE_ROTATE) return set_error(KUSH_ERR_ARG, "kush_sm100_decode_window: unknown flags %d", flags);
     if (window < 1 || sinks < 0)
         return set_error(KUSH_ERR_ARG, "kush_sm100_decode_window: window %d must be >= 1, sinks %d >= 0", window, sinks);
-    return decode_any(head_dim, bits, page, dtype, group, q, out, cache, block_stride, head_stride, tail_k, tail_idx,
-                      block_table, seq_lens, max_pages, hkv, scale, n_splits, part_ml, part_o, n_seqs,
-                      (flags & KUSH_DECODE_ROTATE) ? 1 : 0, order, stream, counters,
-                      window < KUSH_NO_POSITION ? window : KUSH_NO_POSITION, sinks < KUSH_NO_POSITION ? sinks : KUSH_NO_POSITION);
+    const int rot = (flags & KUSH_DECODE_ROTATE) ? 1 : 0;
+    const int rc = decode_any(head_dim, bits, page, dtype, group, q, out, cache, block_stride, head_stride, tail_k, tail_idx,
+                              block_table, seq_lens, max_pages, hkv, scale, n_splits, part_ml, part_o, n_seqs, rot, order,
+                              stream, counters, window < KUSH_NO_POSITION ? window : KUSH_NO_POSITION,
+                              sinks < KUSH_NO_POSITION ? sinks : KUSH_NO_POSITION);
+    if (rc != KUSH_OK || n_splits == 1 || counters) return rc;
+    return rot ? kush_sm100_combine_rotated(head_dim, dtype, group, out, part_ml, part_o, n_splits, hkv, n_seqs, stream)
+               : kush_sm100_combine(head_dim, dtype, group, out, part_ml, part_o, n_splits, hkv, n_seqs, stream);
 }
