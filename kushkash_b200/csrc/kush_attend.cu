@@ -4,7 +4,8 @@
 namespace kush {
 
 // One warp per (row, q head): o = sum_z exp(m_z - M) o_z / sum_z exp(m_z - M) l_z, lane z % 32 holding the factors of its
-// splits, the partial outputs read D/32 channels a lane.  Rows behind the last sequence are left as they are.
+// splits, the partial outputs read D/32 channels a lane.  Rows behind the last sequence (qsl[S]; qsl null: none) are left as
+// they are.
 template <int D, class IN>
 __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out, const float* __restrict__ part_ml,
                                                             const float* __restrict__ part_o, int n_splits, int H, int G,
@@ -13,7 +14,7 @@ __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out
     pdl_wait();
     const int lane = threadIdx.x % WARP;
     const int64_t u = int64_t(blockIdx.x) * 4 + threadIdx.x / WARP;           // (row * H + h) * G + g
-    if (u >= units || u / (H * G) >= qsl[S]) return;
+    if (u >= units || (qsl && u / (H * G) >= qsl[S])) return;
     const int64_t first = (u / G) * n_splits * G + u % G;                    // its partial of split 0; split z at + z G
     float M = -INFINITY;
     for (int z = lane; z < n_splits; z += WARP) M = fmaxf(M, part_ml[2 * (first + int64_t(z) * G)]);
@@ -52,16 +53,16 @@ __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out
     for (int i = 0; i < R; i++) out[u * D + lane * R + i] = from_f32<IN>(o[i] * inv);
 }
 
-static int launch_chunk_combine(int D, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream) {
+int launch_chunk_combine(int D, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream) {
     const int64_t units = rows * a.H * a.G, blocks = (units + 3) / 4;
-    if (blocks > 0x7fffffff) return set_error(KUSH_ERR_ARG, "kush_sm100_attend_chunk: %lld rows", (long long)rows);
+    if (blocks > 0x7fffffff) return set_error(KUSH_ERR_ARG, "attention: %lld rows to merge", (long long)rows);
     return dispatch_dim(D, [&](auto Dc) {
         return dispatch_dtype(dtype, [&](auto in) {
             using IN = decltype(in);
             launch_pdl(chunk_combine_kernel<Dc.value, IN>, dim3(unsigned(blocks)), dim3(128), 0, stream,
                        static_cast<IN*>(a.out), const_cast<const float*>(a.part_ml), const_cast<const float*>(a.part_o),
                        int(a.n_splits), int(a.H), int(a.G), a.qsl, int(a.S), units);
-            return check_launch("kush_sm100_attend_chunk (combine)");
+            return check_launch("attention (combine)");
         });
     });
 }

@@ -134,5 +134,7 @@ __device__ __forceinline__ int64_t part_row(const AttendArgs& a, int64_t row, in
 int attend_tc_supported(int D, int dtype);
 int launch_attend_tc(int D, int bits, int P, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream);
 int launch_attend_simt(int D, int bits, int P, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream);
+// the merge of split partials into a.out (out, part_ml, part_o, n_splits, H, G, qsl, S of a); part_ml 8-byte, part_o 16-byte aligned
+int launch_chunk_combine(int D, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream);
 
 }  // namespace kush

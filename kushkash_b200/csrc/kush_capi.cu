@@ -191,7 +191,19 @@ extern "C" int kush_sm100_decode_window(int32_t head_dim, int32_t bits, int32_t 
                               block_table, seq_lens, max_pages, hkv, scale, n_splits, part_ml, part_o, n_seqs, rot, order,
                               stream, counters, window < KUSH_NO_POSITION ? window : KUSH_NO_POSITION,
                               sinks < KUSH_NO_POSITION ? sinks : KUSH_NO_POSITION);
-    if (rc != KUSH_OK || n_splits == 1 || counters) return rc;
+    if (rc != KUSH_OK || n_splits == 1 || counters || n_seqs == 0) return rc;
+    // a warp per output row reads its splits' factors at once: one sequence, 16 splits: 16.7 -> 16.0 us with the decode
+    if (!rot && aligned16(part_o) && (reinterpret_cast<uintptr_t>(part_ml) & 7) == 0) {
+        AttendArgs a{};
+        a.out = out;
+        a.H = hkv;
+        a.G = group;
+        a.S = n_seqs;
+        a.n_splits = n_splits;
+        a.part_ml = part_ml;
+        a.part_o = part_o;
+        return launch_chunk_combine(head_dim, dtype, a, n_seqs, static_cast<cudaStream_t>(stream));
+    }
     return rot ? kush_sm100_combine_rotated(head_dim, dtype, group, out, part_ml, part_o, n_splits, hkv, n_seqs, stream)
                : kush_sm100_combine(head_dim, dtype, group, out, part_ml, part_o, n_splits, hkv, n_seqs, stream);
 }
