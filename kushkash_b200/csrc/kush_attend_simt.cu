@@ -5,7 +5,9 @@
 // dequantized into shared memory (c * s + b in fp32; tail and new rows as they are; tokens that no row of the tile sees
 // are zeros and neither they nor their pages are read), scores in a 4 x 2 register tile per thread, an online softmax
 // with running maximum and sum per row, then the 4 x D/16 register tile of the output.  Bound by fp32 FMAs and the
-// shared-memory loads that feed them: 2048 rows of 32 q heads over 30001 tokens run at 20 TFLOP/s (51.6 ms).
+// shared-memory loads that feed them: 2 sequences x 100 rows of 32 q heads over 2000
+// int4 tokens in fp32 take 434 us = 15.5 TFLOP/s; a decoded token's rows (fewer than the tile's 32) are bound by the tiles'
+// loads, four tokens of a warp in flight (one sequence, window 8192: 140 us, 151 with one token at a time).
 #include "kush_attend.cuh"
 
 namespace kush {
@@ -79,12 +81,16 @@ __global__ void __launch_bounds__(AS_THREADS) attend_simt_kernel(AttendArgs a) {
     for (int it = i0; it < i1; it++) {
         const int j0 = kt.tile(it) * AS_TN;
         __syncthreads();
-        for (int c = wid; c < AS_TN; c += AS_THREADS / WARP) {               // a warp per token, lanes over channels
-            const int j = j0 + c;
-            float kx[R], vx[R];
+        // a warp per token, lanes over channels, four tokens' loads in flight
+#pragma unroll 1
+        for (int c0 = wid; c0 < AS_TN; c0 += 4 * (AS_THREADS / WARP)) {
+            float kx[4][R], vx[4][R];
 #pragma unroll
-            for (int i = 0; i < R; i++) kx[i] = vx[i] = 0.0f;
-            if (kt.seen(j, t.p1)) {
+            for (int u = 0; u < 4; u++) {
+                const int j = j0 + c0 + u * (AS_THREADS / WARP);
+#pragma unroll
+                for (int i = 0; i < R; i++) kx[u][i] = vx[u][i] = 0.0f;
+                if (!kt.seen(j, t.p1)) continue;
                 if (j < t.ctx) {
                     const uint8_t* rec = a.cache + int64_t(bt[j / P]) * a.block_stride + int64_t(h) * a.head_stride;
                     const int s = j % P;
@@ -92,10 +98,10 @@ __global__ void __launch_bounds__(AS_THREADS) attend_simt_kernel(AttendArgs a) {
 #pragma unroll
                     for (int i = 0; i < R; i++) {
                         const int d = lane + WARP * i;
-                        kx[i] = j < full ? fmaf(float(code_at<D, BITS>(rec + s * F::DC, d)), h_load(rec + F::OFF_KS, d),
-                                                h_load(rec + F::OFF_KB, d))
-                                         : to_f32(tail[s * D + d]);
-                        vx[i] = fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + s * F::DC, d)), vsc, vbi);
+                        kx[u][i] = j < full ? fmaf(float(code_at<D, BITS>(rec + s * F::DC, d)), h_load(rec + F::OFF_KS, d),
+                                                   h_load(rec + F::OFF_KB, d))
+                                            : to_f32(tail[s * D + d]);
+                        vx[u][i] = fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + s * F::DC, d)), vsc, vbi);
                     }
                 } else {
                     const int64_t row = t.q0 + (j - t.ctx);
@@ -103,15 +109,19 @@ __global__ void __launch_bounds__(AS_THREADS) attend_simt_kernel(AttendArgs a) {
                     const IN* vn = static_cast<const IN*>(a.v_new) + row * a.v_stride + int64_t(h) * D;
 #pragma unroll
                     for (int i = 0; i < R; i++) {
-                        kx[i] = to_f32(kn[lane + WARP * i]);
-                        vx[i] = to_f32(vn[lane + WARP * i]);
+                        kx[u][i] = to_f32(kn[lane + WARP * i]);
+                        vx[u][i] = to_f32(vn[lane + WARP * i]);
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < R; i++) {
-                ks[c * QP + lane + WARP * i] = kx[i];
-                vs[c * D + lane + WARP * i] = vx[i];
+            for (int u = 0; u < 4; u++) {
+                const int c = c0 + u * (AS_THREADS / WARP);
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    ks[c * QP + lane + WARP * i] = kx[u][i];
+                    vs[c * D + lane + WARP * i] = vx[u][i];
+                }
             }
         }
         __syncthreads();

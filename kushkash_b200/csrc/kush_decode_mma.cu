@@ -376,8 +376,8 @@ __device__ __noinline__ void combine_if_last(int32_t* counters, int64_t sh, int 
 // grid (S, Hkv, n_splits), block 128.  ROT: q rotated in the prologue and the output rotated back before its store;
 // ORD: CTA x works on sequence order[x] (separate instantiations, so the plain kernels keep their code).
 // WIN: a sliding window with sink tokens.  The page loop walks the sequence's visible pages (VisiblePages) and reads no
-// other page nor its block-table entry; a 16-token tile with no visible token is skipped, and in the at most three tiles
-// that a border cuts the masked tokens' scores become -inf.  Every tile that is processed holds a visible token, so the
+// other page nor its block-table entry; in the (at most two) pages that a border cuts a 16-token tile with no visible token
+// is skipped and masked tokens' scores become -inf.  Every tile that is processed holds a visible token, so the
 // running max is finite after its first tile.  kb_ref is the K bias of the first visible page, for all splits alike.
 template <int D, int BITS, int P, int NT, class IN, bool ROT, bool ORD, bool WIN>
 __global__ void __launch_bounds__(MMA_NW * WARP, (MmaCfg<D, BITS, P, NT>::MINB)) decode_mma_kernel(
