@@ -12,17 +12,42 @@ from dataclasses import dataclass
 import torch
 
 
+# keys that every type allows without reading them (rope_theta is compared), and those that each reads
+_COMMON_KEYS = {"rope_type", "type", "rope_theta", "original_max_position_embeddings", "finetuned"}
+_KEYS = {"default": set(), "linear": {"factor"}, "ntk": {"factor"},
+         "yarn": {"factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"},
+         "llama3": {"factor", "low_freq_factor", "high_freq_factor"}}
+
+
+def _yarn_factor(factor: float, scaling: dict) -> float:
+    """The factor of the cosines and sines under yarn scaling."""
+    def grow(m: float) -> float:
+        return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+    if "attention_factor" in scaling:
+        return float(scaling["attention_factor"])
+    mscale, all_dim = float(scaling.get("mscale", 0)), float(scaling.get("mscale_all_dim", 0))
+    if mscale and all_dim:
+        return grow(mscale) / grow(all_dim)
+    if all_dim or mscale not in (0.0, 1.0):       # (1 alone is the default's own factor)
+        raise ValueError("rotary: mscale and mscale_all_dim go together")
+    return grow(1.0)
+
+
 def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None) -> tuple[list[float], float]:
     """(radians per position of pair i, factor of the cosines and sines).  Base frequencies theta^(-2i / rotary_dim);
     `scaling` stretches them for contexts longer than the trained one, in the keys model configurations use:
       rope_type "linear"   factor: every frequency divided by it
                 "ntk"      factor: theta becomes theta * factor^(r / (r - 2)): the fastest pair unchanged, the slowest / factor
-                "yarn"     factor, original_max_position_embeddings [, beta_fast 32, beta_slow 1, attention_factor
-                           0.1 ln(factor) + 1]: pairs that turn more than beta_fast times over the original context kept,
-                           those below beta_slow divided by factor, a ramp over the pair's index between
+                "yarn"     factor, original_max_position_embeddings [, beta_fast 32, beta_slow 1, truncate True]: pairs that
+                           turn more than beta_fast times over the original context kept, those below beta_slow divided
+                           by factor, a ramp over the pair's index between (its ends whole indices unless truncate is
+                           False); the factor of cosines and sines is attention_factor, or from mscale and mscale_all_dim
+                           (0.1 mscale ln(factor) + 1) / (0.1 mscale_all_dim ln(factor) + 1), or 0.1 ln(factor) + 1
                 "llama3"   factor, low_freq_factor, high_freq_factor, original_max_position_embeddings: the same with a ramp
                            over the number of turns
-                "default"  none"""
+                "default"  none
+    A key given as None counts as absent; rope_theta has to be theta; a key that the type does not read is refused."""
     if theta <= 0:
         raise ValueError(f"rotary: theta must be positive, got {theta}")
     r = rotary_dim
@@ -30,6 +55,14 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
     if not scaling:
         return freq, 1.0
     kind = scaling.get("rope_type", scaling.get("type"))
+    if kind not in _KEYS:
+        raise ValueError(f"rotary: unknown scaling {kind!r} (linear, ntk, yarn, llama3 or default)")
+    scaling = {key: value for key, value in scaling.items() if value is not None}
+    unread = sorted(set(scaling) - _COMMON_KEYS - _KEYS[kind])
+    if unread:
+        raise ValueError(f"rotary: {kind} scaling does not know {', '.join(unread)}")
+    if float(scaling.get("rope_theta", theta)) != theta:
+        raise ValueError(f"rotary: rope_theta {scaling['rope_theta']} of the scaling is not theta {theta}")
     try:
         if kind == "default":
             return freq, 1.0
@@ -49,22 +82,19 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
             context = float(scaling["original_max_position_embeddings"])
             at = [r * math.log(context / (beta * 2 * math.pi)) / (2 * math.log(theta))
                   for beta in (float(scaling.get("beta_fast") or 32), float(scaling.get("beta_slow") or 1))]
-            lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), r - 1)
+            if scaling.get("truncate", True):
+                at = [math.floor(at[0]), math.ceil(at[1])]
+            lo, hi = max(at[0], 0), min(at[1], r - 1)
             keep = [1 - min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0) for i in range(r // 2)]
-            scale = scaling.get("attention_factor")
-            if scale is None:
-                scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
-            return [f / factor * (1 - w) + f * w for f, w in zip(freq, keep)], float(scale)
-        if kind == "llama3":
-            context = float(scaling["original_max_position_embeddings"])
-            low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
-            if high <= low:
-                raise ValueError("rotary: high_freq_factor must be above low_freq_factor")
-            keep = [min(max((context * f / (2 * math.pi) - low) / (high - low), 0.0), 1.0) for f in freq]
-            return [f / factor * (1 - w) + f * w for f, w in zip(freq, keep)], 1.0
+            return [f / factor * (1 - w) + f * w for f, w in zip(freq, keep)], _yarn_factor(factor, scaling)
+        context = float(scaling["original_max_position_embeddings"])          # llama3
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if high <= low:
+            raise ValueError("rotary: high_freq_factor must be above low_freq_factor")
+        keep = [min(max((context * f / (2 * math.pi) - low) / (high - low), 0.0), 1.0) for f in freq]
+        return [f / factor * (1 - w) + f * w for f, w in zip(freq, keep)], 1.0
     except KeyError as e:
         raise ValueError(f"rotary: {kind} scaling needs {e.args[0]}") from None
-    raise ValueError(f"rotary: unknown scaling {kind!r} (linear, ntk, yarn, llama3 or default)")
 
 
 @dataclass(frozen=True)
