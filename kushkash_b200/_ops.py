@@ -320,15 +320,16 @@ class Ops:
         kernel and the output rotated back before its store.  order: a contiguous int32 permutation of the
         sequences, CTA x then decoding sequence order[x] (longest_first()); the outputs do not depend on it.
         window: the query sees the last `window` tokens (its own among them) and the first `sinks`; pages without a
-        visible token are not read, nor their block-table entries (give splits() the same window and sinks)."""
+        visible token are not read, nor their block-table entries (give splits() the same window and sinks).  Under a
+        window the arguments are checked: q and out contiguous [S, H * G, D], int32 index tensors of at least S rows."""
+        if window is not None or sinks:
+            self._decode_window(q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, work, rotate, order,
+                                fused, window, sinks)
+            return
         S, H = q.shape[0], tail_k.shape[1]
         ml = o = 0
         if n_splits > 1:
             ml, o = self._parts(S, H, n_splits, work, fused)
-        if window is not None or sinks:
-            self._decode_window(q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale, n_splits, ml, o, rotate,
-                                order, fused, window, sinks)
-            return
         if fused and n_splits > 1:
             if order is not None:
                 _need(order.dtype == torch.int32 and order.numel() == S and order.is_contiguous(),
@@ -371,21 +372,41 @@ class Ops:
         self._run("kush_sm100_decode_ex", *head, 1 if rotate else 0, order.data_ptr())
 
     def _decode_window(self, q, out, cache, block_table, seq_lens, tail_idx, tail_k, scale: float, n_splits: int,
-                       part_ml: int, part_o: int, rotate: bool, order: torch.Tensor | None, fused: bool,
-                       window: int | None, sinks: int) -> None:
-        S, H = q.shape[0], tail_k.shape[1]
-        self._here("decode", q, out, cache, block_table, seq_lens, tail_idx, tail_k)
+                       work: torch.Tensor | None, rotate: bool, order: torch.Tensor | None, fused: bool, window: int | None,
+                       sinks: int) -> None:
+        D, dt, i32, shape, tail = self.D, self.dtype, torch.int32, q.shape, tail_k.shape
+        self._here("decode", q, out, cache, block_table, seq_lens, tail_idx, tail_k,
+                   *(t for t in (work, order) if t is not None))
         if window is None or window < 1 or sinks < 0:
             raise ValueError(f"decode: window must be >= 1 and sinks >= 0 (sinks need a window), got {window} and {sinks}")
+        if not (q.dtype == out.dtype == tail_k.dtype == dt):
+            raise ValueError(f"decode: q, out and tail_k must be {dt}")
+        if len(tail) != 4 or tail[2] != self.P or tail[3] != D or not tail_k.is_contiguous():
+            raise ValueError(f"decode: tail_k must be contiguous [slots, H, {self.P}, {D}]")
+        S, H = shape[0], tail[1]
+        if len(shape) != 3 or shape[1] != H * self.G or shape[2] != D or out.shape != shape or not (
+                q.is_contiguous() and out.is_contiguous()):
+            raise ValueError(f"decode: q and out must be contiguous [S, {H * self.G}, {D}] (a part of q|k|v rows: its .contiguous())")
+        if (not (seq_lens.dtype == tail_idx.dtype == block_table.dtype == i32)
+                or seq_lens.dim() != 1 or tail_idx.dim() != 1 or block_table.dim() != 2
+                or min(seq_lens.shape[0], tail_idx.shape[0], block_table.shape[0]) < S
+                or not seq_lens.is_contiguous() or not tail_idx.is_contiguous() or block_table.stride(1) != 1):
+            raise ValueError("decode: seq_lens and tail_idx must be contiguous int32 [S], block_table [S, pages] int32 with "
+                             "contiguous rows")
+        if cache.dim() < 2 or cache.shape[1] < H:
+            raise ValueError(f"decode: cache must hold the records of {H} kv heads, got {tuple(cache.shape)}")
+        part_ml = part_o = counters = address = None
+        if n_splits > 1:
+            part_ml, part_o = self._parts(S, H, n_splits, work, fused)
+            counters = part_ml + 4 * S * H * n_splits * self.G * (D + 2) if fused else None
         if order is not None:
-            _need(order.dtype == torch.int32 and order.numel() == S and order.is_contiguous(),
+            _need(order.dtype == i32 and order.numel() == S and order.is_contiguous(),
                   "decode: order must be a contiguous int32 permutation of the sequences")
-        counters = part_ml + 4 * S * H * n_splits * self.G * (self.D + 2) if fused and n_splits > 1 else None
+            address = order.data_ptr()
         self._run("kush_sm100_decode_window", *self._fmt, self.G, q.data_ptr(), out.data_ptr(), *_pool(cache),
-                  tail_k.data_ptr(), tail_idx.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-                  block_table.stride(0), H, float(scale), n_splits, part_ml or None, part_o or None, counters, S,
-                  1 if rotate else 0, order.data_ptr() if order is not None else None, min(window, _I32_MAX),
-                  min(sinks, _I32_MAX))
+                  tail_k.data_ptr(), tail_idx.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), block_table.stride(0),
+                  H, float(scale), n_splits, part_ml, part_o, counters, S, 1 if rotate else 0, address,
+                  min(window, _I32_MAX), min(sinks, _I32_MAX))
 
     # ---------------------------------------------------------------- chunk attention
     def chunk_splits(self, num_rows: int, num_seqs: int, num_kv_heads: int, max_len: int, *, window: int | None = None,
