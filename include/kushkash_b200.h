@@ -189,7 +189,7 @@ int kush_sm100_decode_window(int32_t head_dim, int32_t bits, int32_t page, int32
  * the positions up to its own; with window > 0 of those only the last `window` (its own among them) and the first
  * `sinks`.  History keys are c * ks + kb, the unfinished page's exact ones from tail_k[tail_idx[s]]; history values
  * c * vs + vb; new rows enter as they are.  Pages that no row of the chunk sees are not read, nor their block-table
- * entries.  Rows at and behind query_start_loc[n_seqs] are neither read nor written.
+ * entries.  Rows before query_start_loc[0] and from query_start_loc[n_seqs] on are neither read nor written.
  * n_splits > 1 divides each row tile's keys over that many blocks and merges them with a second kernel: part_ml
  * [n_rows][hkv][n_splits][group][2], part_o [n_rows][hkv][n_splits][group][head_dim] fp32. */
 int kush_sm100_attend_chunk(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group, const void *q,

@@ -430,7 +430,7 @@ class Ops:
         (no unpacked copy); call it before write() stores the rows.  Sequence s owns rows [qsl[s], qsl[s+1]) of q
         [rows, H * G, D], k and v [rows, H, D] (row strides free, head stride D) and out [rows, H * G, D]
         (contiguous); seq_lens[s] counts them, as in write().  Any mix of chunk lengths, one token and no history
-        included; rows at and behind qsl[S] are left alone.  window, sinks: as in decode(), for every row from its own
+        included; rows before qsl[0] and from qsl[S] on are left alone.  window, sinks: as in decode(), for every row from its own
         position.  n_splits > 1 (chunk_splits()) divides each tile's keys over more blocks and needs `work`
         (chunk_work_size() fp32 elements).  Over a rotated cache, give it fwht() of q, k and v (write() wants the
         latter two as well) and take fwht() of out."""

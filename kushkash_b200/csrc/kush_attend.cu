@@ -4,8 +4,8 @@
 namespace kush {
 
 // One warp per (row, q head): o = sum_z exp(m_z - M) o_z / sum_z exp(m_z - M) l_z, lane z % 32 holding the factors of its
-// splits, the partial outputs read D/32 channels a lane.  Rows behind the last sequence (qsl[S]; qsl null: none) are left as
-// they are.
+// splits, the partial outputs read D/32 channels a lane.  Rows before the first sequence and behind the last one (before
+// qsl[0], from qsl[S] on; qsl null: none) have no partials and are left as they are.
 template <int D, class IN>
 __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out, const float* __restrict__ part_ml,
                                                             const float* __restrict__ part_o, int n_splits, int H, int G,
@@ -14,7 +14,8 @@ __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out
     pdl_wait();
     const int lane = threadIdx.x % WARP;
     const int64_t u = int64_t(blockIdx.x) * 4 + threadIdx.x / WARP;           // (row * H + h) * G + g
-    if (u >= units || (qsl && u / (H * G) >= qsl[S])) return;
+    if (u >= units) return;
+    if (const int64_t row = u / (H * G); qsl && (row < qsl[0] || row >= qsl[S])) return;
     const int64_t first = (u / G) * n_splits * G + u % G;                    // its partial of split 0; split z at + z G
     float M = -INFINITY;
     for (int z = lane; z < n_splits; z += WARP) M = fmaxf(M, part_ml[2 * (first + int64_t(z) * G)]);
