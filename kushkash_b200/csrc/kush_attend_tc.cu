@@ -14,8 +14,12 @@
 // K' = c ks + (kb - ref), fp16, ref = the key bias of the first finished page the block sees: the same shift of every
 // score of a row, which the softmax drops; large channel offsets are gone before the rounding to fp16.  q and the new
 // rows enter as fp16 too (exact for bf16 within fp16's range, which the cache's own fp16 scales have as well).  Scores,
-// maxima, sums and outputs stay fp32; the weights p = 2^(s - m) <= 2^8 are rounded once to fp16.  The maximum moves
-// lazily: O is rescaled only when a score passes the maximum in use by 2^8.
+// maxima, sums and outputs stay fp32.  The maximum m in use moves lazily: O is rescaled only when a score passes it by
+// 2^TAU.  The weights enter the products as fp16, p = 2^(s - m + TC_UP) <= 2^(TAU + TC_UP) = 2^15: the upper end of fp16's
+// range, so that a weight keeps its 11 bits down to 2^-23 of the row's largest and an absolute step of 2^-33 below.  (With the
+// largest at 1, under a sink token whose value is near zero, the weights that make the output fell among fp16's subnormals;
+// those e^-17.3 below the sink's were lost.)  Weights of a tile that the maximum moves past are rounded a second time.
+// TAU = 4, 5, 6, 8 (steps 2^-35, 2^-34, 2^-33, 2^-31): ragged prefill 465, 462, 460, 455 us, windowed int8 338, 327, 325, 324.
 //
 // What bounds it.  A pair of 128-row tiles and a key tile are 32 products of 64 cycles (2048 cycles of tensor cores), 32768
 // exponentials at 16 a cycle (2048 cycles) and 32768 dequantized values, all on four schedulers: none of the three alone,
@@ -45,7 +49,7 @@
 namespace kush {
 
 constexpr int TC_TM = 256, TC_TN = 128, TC_THREADS = 16 * WARP, TC_NPROD = 6;
-constexpr float TC_TAU = 8.0f;
+constexpr float TC_TAU = 6.0f, TC_UP = 15.0f - TC_TAU;
 
 __device__ int g_attend_error = 0;
 
@@ -383,7 +387,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     if (up) m = mx;
                     la = __fmul2_rn(la, make_float2(corr, corr));
                     lb = __fmul2_rn(lb, make_float2(corr, corr));
-                    const __half2 ch = __float2half2_rn(corr);
 #pragma unroll 1
                     for (int e = 0; e < (n > 0 ? D / 32 : 0); e++) {               // O (the slot's last product is done)
                         uint32_t x[32];
@@ -401,8 +404,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                         wait_ld(x);
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&x[i]), ch);
-                            p[i] = *reinterpret_cast<const uint32_t*>(&h);
+                            const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
+                            p[i] = pack_h2(w.x * corr, w.y * corr);            // (corr itself may be below fp16's range)
                         }
                         tmem_st16(s_at + 16 * e, p);
                         wait_st();
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 // dependence between them, under which the next piece's maximum is taken), its sum and its P
                 auto piece = [&](int c, uint32_t (&x)[32], uint32_t (&y)[32], float mx, auto last) -> float {
                     if (__any_sync(0xffffffffu, mx > m + TC_TAU)) move_max(c, mx); // (m = -inf: any score)
-                    const float mm = m == -INFINITY ? 0.0f : -m;                   // nothing seen yet: weights 0
+                    const float mm = m == -INFINITY ? 0.0f : TC_UP - m;            // nothing seen yet: weights 0
                     const float2 sc2 = make_float2(sc, sc), mm2 = make_float2(mm, mm);
                     if constexpr (!decltype(last)::value) tmem_ld32(s_at + 32 * c + 32, y);
 #pragma unroll
@@ -540,7 +543,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 }
             }
             if (real && a.n_splits > 1) {
-                a.part_ml[2 * pr] = ok ? m * 0.69314718055994531f : 0.0f;         // log2 units -> natural, for the combine
+                // sum and output are in units of 2^(m - TC_UP); log2 units -> natural, for the combine
+                a.part_ml[2 * pr] = ok ? (m - TC_UP) * 0.69314718055994531f : 0.0f;
                 a.part_ml[2 * pr + 1] = l;
             }
         }

@@ -4,6 +4,7 @@ import torch
 
 from attend_ref import Cache, check
 from test_gpu_attend import Step, ops_of
+from tolerance import half_ulp
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +27,51 @@ def test_rows_before_the_first_sequence(D, dtype, n_splits):
     own = Step(c, [9, 140], seed=2, spare=0)
     own.q, own.k, own.v = (t[3:152] for t in (step.q, step.k, step.v))
     check(out[3:152], *own.reference(None, 0), dtype, f"rows 3.. splits {n_splits}")
+
+
+def exact_rows(q, k, v, scale, seen, up):
+    """softmax(q k) v of one head in 64 bits, and the bound of a kernel that takes these operands exactly (bf16 or fp16 values
+    within fp16's normal range), adds scores in fp32 (D terms and the scale: D + 16 roundings) and rounds weights to fp16
+    twice at most: 2^-11 relative each, or 2^-25 of a unit that is 2^up below the largest weight."""
+    q, k, v = q.double().cpu(), k.double().cpu(), v.double().cpu()
+    s = (q @ k.T * scale).masked_fill(~seen, -torch.inf)
+    ds = ((q.abs() @ k.abs().T) * abs(scale) * (q.shape[1] + 16) * 2.0 ** -24).masked_fill(~seen, 0).amax(-1)
+    w = torch.softmax(s, dim=-1)
+    small = (seen.double() @ v.abs()) * (2 * 2.0 ** -25 * 2.0 ** -up * w.amax(-1))[:, None]
+    return w @ v, (w @ v.abs()) * (2 * 2.0 ** -11 + 2 * ds[:, None] + 2.0 ** -20) + small
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("n,at,window", [(100, 40, None), (100, 0, None), (300, 200, None), (3000, 0, None), (3000, 1, 2000), (1500, 1400, None)])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 17.3, 18.5])
+def test_small_weights_beside_one_large_one(dtype, D, n, at, window, gap):
+    """One token scores `gap` above all others and has the value zero (an attention sink): the output is made of the
+    small weights, wherever in the tiles the large one stands."""
+    ops = ops_of(D, 4, 1, dtype, 16)
+    c = Cache(ops, [0], 1, seed=1)
+    g = torch.Generator().manual_seed(n + at)
+    side = torch.sign(torch.randn(D, generator=g))
+    k = 0.05 * torch.randn(n, 1, D, generator=g)
+    v = 0.5 + torch.rand(n, 1, D, generator=g)
+    q = (1.0 + torch.rand(n, 1, D, generator=g)) * side
+    scale = D ** -0.5
+    k[at, 0] = side * gap / (1.5 * D * scale)
+    v[at] = 0.0
+    q, k, v = (t.to(dtype).cuda() for t in (q, k, v))
+    qsl, lens = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, n], [n]))
+    rows = torch.arange(max(at, n - 70), n)
+    j = torch.arange(n)
+    seen = j[None] <= rows[:, None]
+    if window is not None:
+        seen &= (j[None] > rows[:, None] - window) | (j[None] < at + 1)
+    want, bound = exact_rows(q[rows, 0], k[:, 0], v[:, 0], scale, seen, 9)
+    for n_splits in (1, 3):
+        work = torch.full((ops.chunk_work_size(n, 1, n_splits),), float("nan"), device="cuda")
+        out = torch.empty_like(q)
+        ops.attend_chunk(q, k, v, out, qsl, lens, c.tail_idx, c.pool, c.block_table, c.tail_k, scale, n_splits, work, window=window,
+                         sinks=at + 1 if window else 0)
+        # (element by element, without check()'s relative norm: an fp16 output of 100 e^-18.5 = 9e-7 has a half step of 2^-25, 3%)
+        got = out[rows, 0].double().cpu()
+        worst = ((got - want).abs() / (bound + half_ulp(want.abs() + bound, dtype))).max().item()
+        print(f"gap {gap} at {at} of {n} splits {n_splits}: {worst:.3f} of the bound")
+        assert worst <= 1.0, f"{worst:.2f} times the bound"
