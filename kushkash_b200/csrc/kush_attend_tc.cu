@@ -11,9 +11,12 @@
 //   S[128 x 128] = Q K'^T   (both from shared memory, K-major, 128-byte swizzle), fp32 in TMEM
 //   O[128 x D]  += P V      (P fp16 in TMEM over the first half of S's columns, V from shared memory, N-major)
 // (softmax warps that have no rows bring keys and values too: 20 rows of drafted tokens leave six of them.)
-// K' = c ks + (kb - ref), fp16, ref = the key bias of the first finished page the block sees: the same shift of every
-// score of a row, which the softmax drops; large channel offsets are gone before the rounding to fp16.  q and the new
-// rows enter as fp16 too (exact for bf16 within fp16's range, which the cache's own fp16 scales have as well).  Scores,
+// Keys of records enter as K' = c ks + (kb - ref), fp16, ref = the key bias of the first finished page the block sees: a shift
+// of a row's scores by q ref, and large channel offsets are gone before the rounding to fp16.  The unfinished page's keys and
+// the new rows enter as they are (exact for fp16, and for bf16 from 2^-17 to 65504; smaller ones as multiples of 2^-24), as q
+// and new values do; q ref, in fp32, is taken off their scores.  (Shifted and rounded as the records' are they cost fp16 rows
+// three quarters of their error: 7.6e-4 relative against 3.6e-4, windowed int8.)  Values of records are c vs + vb rounded to
+// fp16: the products take one type of operand, and both factors apart would cost the softmax two operations a weight.  Scores,
 // maxima, sums and outputs stay fp32.  The maximum m in use moves lazily: O is rescaled only when a score passes it by
 // 2^TAU.  The weights enter the products as fp16, p = 2^(s - m + TC_UP) <= 2^(TAU + TC_UP) = 2^15: the upper end of fp16's
 // range, so that a weight keeps its 11 bits down to 2^-23 of the row's largest and an absolute step of 2^-33 below.  (With the
@@ -287,11 +290,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     const uint8_t* hcache = a.cache + int64_t(h) * a.head_stride;
     const int full = t.ctx / P * P;                                                // cached tokens in finished pages
     // the key reference: the bias of the first finished page that the row tile sees (the same for all its splits)
-    {
-        const int first = kt.a > 0 ? 0 : kt.lo / P * P;
-        const bool have = first < full;
-        const uint8_t* rec = have ? hcache + int64_t(bt[first / P]) * a.block_stride : nullptr;
-        if (tid < D) ref[tid] = have ? h_load(rec + F::OFF_KB, tid) : 0.0f;
+    const int first = kt.a > 0 ? 0 : kt.lo / P * P;
+    const bool have_ref = first < full;
+    if (tid < D) {
+        const uint8_t* rec = have_ref ? hcache + int64_t(bt[first / P]) * a.block_stride : nullptr;
+        ref[tid] = have_ref ? h_load(rec + F::OFF_KB, tid) : 0.0f;
     }
     // query rows to fp16, negated under a negative scale (the softmax multiplies by its magnitude)
     {
@@ -338,6 +341,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         const float sc = fmaxf(fabsf(a.sm_log2), 1e-30f);                          // (a masked score stays -inf under scale 0)
         const uint32_t lanes = uint32_t(wrow) << 16;
         const uint32_t s_at = tmem + lanes + 128 * slot, o_at = tmem + lanes + 256 + 128 * slot;
+        float qref = 0.0f;                                                         // q ref: the shift of the records' scores
+        if (have_ref) {
+            const uint8_t* qr = sm + M::Q + (paired ? slot * M::TILE : 0);
+#pragma unroll 1
+            for (int c = 0; c < CH; c++) {
+                const uint4 raw = *reinterpret_cast<const uint4*>(qr + tile_off(row, c));
+                const __half2* e = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 x = __half22float2(e[i]);
+                    qref = fmaf(x.x, ref[8 * c + 2 * i], qref);
+                    qref = fmaf(x.y, ref[8 * c + 2 * i + 1], qref);
+                }
+            }
+        }
         float m = -INFINITY;                                                       // the maximum in use, log2 units
         float2 la = make_float2(0.0f, 0.0f), lb = la;                              // the weights' sum, in four parts
         int n = 0;                                                                 // tiles done by this slot
@@ -362,8 +380,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 const int j0 = kt.tile(it) * TC_TN;
                 // columns [0, hi] seen, and of those [lo, ...) or [0, sk)
                 const int hi = pos - j0, lo = a.window > 0 ? pos - a.window + 1 - j0 : -1, sk = a.sinks - j0;
+                // columns from `exact` on hold unshifted keys: q ref comes off them here, or (all columns) with the maximum
+                const int exact = have_ref ? full - j0 : TC_TN;
+                const float shift = exact <= 0 ? -qref * sc : 0.0f;
                 const bool cut = j0 + TC_TN - 1 > wp0 || (a.window > 0 && j0 < wp1 - a.window + 1 && j0 + TC_TN > a.sinks);
                 // (loops over 32-column pieces stay rolled: five roles' code shares the instruction caches)
+                if (exact > 0 && exact < TC_TN) {                                  // once in a row's walk
+#pragma unroll 1
+                    for (int c = exact / 32; c < 4; c++) {
+                        uint32_t x[32];
+                        tmem_ld32(s_at + 32 * c, x);
+                        wait_ld(x);
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (32 * c + i >= exact) x[i] = __float_as_uint(__uint_as_float(x[i]) - qref);
+                        tmem_st32(s_at + 32 * c, x);
+                    }
+                    wait_st();
+                }
                 if (cut) {                                                         // masked scores become -inf in TMEM
 #pragma unroll 1
                     for (int c = 0; c < 4; c++) {
@@ -419,13 +453,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                     for (int i = 8; i < 32; i += 8)
 #pragma unroll
                         for (int k = 0; k < 4; k++) m4[k] = max3(m4[k], __uint_as_float(x[i + k]), __uint_as_float(x[i + k + 4]));
-                    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                    return fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), sc, shift);
                 };
                 // the weights of piece c in place of its scores (first the differences, then all 32 exponentials without a
                 // dependence between them, under which the next piece's maximum is taken), its sum and its P
                 auto piece = [&](int c, uint32_t (&x)[32], uint32_t (&y)[32], float mx, auto last) -> float {
                     if (__any_sync(0xffffffffu, mx > m + TC_TAU)) move_max(c, mx); // (m = -inf: any score)
-                    const float mm = m == -INFINITY ? 0.0f : TC_UP - m;            // nothing seen yet: weights 0
+                    const float mm = m == -INFINITY ? 0.0f : TC_UP - m + shift;    // nothing seen yet: weights 0
                     const float2 sc2 = make_float2(sc, sc), mm2 = make_float2(mm, mm);
                     if constexpr (!decltype(last)::value) tmem_ld32(s_at + 32 * c + 32, y);
 #pragma unroll
@@ -660,12 +694,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                             y[k] = kv ? fmaf(float(code_at<D, BITS>(rec + F::OFF_VQ + at * F::DC, d)), h_load(rec + F::OFF_VS, at),
                                              h_load(rec + F::OFF_VB, at))
                                       : fmaf(float(code_at<D, BITS>(rec + at * F::DC, d)), h_load(rec + F::OFF_KS, d),
-                                             h_load(rec + F::OFF_KB, d));
+                                             h_load(rec + F::OFF_KB, d) - ref[d]);
                         }
-                    }
-                    if constexpr (!kv) {
-#pragma unroll
-                        for (int k = 0; k < 8; k++) y[k] -= ref[8 * cc + k];
                     }
                 }
                 st_chunk(dst + tile_off(row, cc), pack_h2(y[0], y[1]), pack_h2(y[2], y[3]), pack_h2(y[4], y[5]), pack_h2(y[6], y[7]));
@@ -710,21 +740,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 mixed(kvc, j0, kind, dst);
                 return;
             }
-            const float4 ra = *reinterpret_cast<const float4*>(ref + 8 * cc), rb = *reinterpret_cast<const float4*>(ref + 8 * cc + 4);
-            const float2 minus[4] = {make_float2(-ra.x, -ra.y), make_float2(-ra.z, -ra.w), make_float2(-rb.x, -rb.y), make_float2(-rb.z, -rb.w)};
 #pragma unroll
             for (int i = 0; i < NI; i++) {
                 uint32_t p[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const uint32_t e = r[4 * i + k];                               // two channels
-                    if constexpr (std::is_same_v<IN, __half>) {
-                        p[k] = kv ? e : h2_sub(e, pack_h2(-minus[k].x, -minus[k].y));
-                    } else {
-                        float2 y = make_float2(__uint_as_float(e << 16), __uint_as_float(e & 0xFFFF0000u));
-                        if constexpr (!kv) y = __fadd2_rn(y, minus[k]);
-                        p[k] = pack_h2(y.x, y.y);
-                    }
+                    if constexpr (std::is_same_v<IN, __half>) p[k] = e;
+                    else p[k] = pack_h2(__uint_as_float(e << 16), __uint_as_float(e & 0xFFFF0000u));
                 }
                 // (rows RPI apart: the swizzle's upper bits)
                 const uint32_t flip = RPI == 2 ? (i & 3) << 5 : (i & 1) << 6;

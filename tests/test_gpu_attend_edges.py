@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from attend_ref import Cache, check
+from attend_ref import Cache, check, dequantize
 from test_gpu_attend import Step, ops_of
 from tolerance import half_ulp
 
@@ -75,3 +75,50 @@ def test_small_weights_beside_one_large_one(dtype, D, n, at, window, gap):
         worst = ((got - want).abs() / (bound + half_ulp(want.abs() + bound, dtype))).max().item()
         print(f"gap {gap} at {at} of {n} splits {n_splits}: {worst:.3f} of the bound")
         assert worst <= 1.0, f"{worst:.2f} times the bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,bits,P,ctx,new,window,sinks", [(128, 4, 16, 70, 12, None, 0), (128, 8, 32, 300, 200, None, 0),
+                                                           (64, 4, 16, 128, 140, None, 0), (64, 8, 32, 261, 30, 100, 3),
+                                                           (128, 8, 16, 5, 40, None, 0)])
+def test_new_and_unfinished_keys_enter_as_they_are(dtype, D, bits, P, ctx, new, window, sinks):
+    """Finished pages whose keys lie about 4000 in two channels, before new rows that do not: the new rows' keys must not lose
+    what a shift by the pages' bias would round off.  q takes the two channels with opposite signs, so that the scores of the
+    history stay small."""
+    ops = ops_of(D, bits, 2, dtype, P)
+    c = Cache(ops, [ctx], 1, seed=7, pad_blocks=8)
+    g = torch.Generator().manual_seed(ctx + new)
+    k = torch.randn(ctx, 1, D, generator=g)
+    k[:, :, 4:6] += 4000
+    k, v = k.to(dtype).cuda(), torch.randn(ctx, 1, D, generator=g).to(dtype).cuda()
+    qsl = torch.tensor([0, ctx], dtype=torch.int32, device="cuda")
+    js, jp, _ = ops.write_jobs(qsl, c.seq_lens, ctx // P + 2)
+    ops.write(k, v, qsl, c.seq_lens, c.tail_idx, js, jp, c.pool, c.block_table, c.tail_k)
+    torch.cuda.synchronize()
+    c.k_all, c.v_all, c.kb_all = dequantize(c.pool, D, bits, P)
+    c.tail_cpu = c.tail_k.cpu()
+    step = Step(c, [new], seed=3, spare=0)
+    step.q[:, :, 4], step.q[:, :, 5] = 8.0, -8.0
+    kh, vh = c.tokens(0)
+    full = ctx // P * P
+    K, V = torch.cat([kh, step.k.cpu().double()])[:, 0], torch.cat([vh, step.v.cpu().double()])[:, 0]
+    first = 0 if sinks or window is None else (ctx - window + 1) // P * P
+    ref = c.kb_all[int(c.table_cpu[0, first // P]), 0] if full else torch.zeros(D, dtype=torch.float64)
+    pos, j = ctx + torch.arange(new), torch.arange(ctx + new)
+    seen = j[None] <= pos[:, None]
+    if window is not None:
+        seen &= (j[None] > pos[:, None] - window) | (j[None] < sinks)
+    q = step.q.cpu().double().transpose(0, 1).reshape(-1, D)                   # [2 heads, rows]
+    see = seen.repeat(2, 1)
+    w = torch.softmax((q @ K.T * D ** -0.5).masked_fill(~see, -torch.inf), -1)
+    # the records' keys are rounded to fp16 three times after the shift (bias - ref, c ks + that, and q is exact); every score
+    # adds D terms of the unshifted size in fp32 (the shift among them), twice
+    ds = (q.abs() @ (K - ref).abs().T * 3 * 2.0 ** -11 * (j < full) + 2 * (q.abs() @ K.abs().T) * (D + 16) * 2.0 ** -24) * D ** -0.5
+    ds = ds.masked_fill(~see, 0)
+    # w_j e^d_j / sum_i w_i e^d_i with |d| <= ds is off by a factor of at most e^ds_j sum_i w_i e^ds_i; weights and values are
+    # rounded twice and once to fp16
+    move = ds.exp() * (w * ds.exp()).sum(-1, keepdim=True) * (1 + 3 * 2.0 ** -11) - 1
+    bound = (w * move) @ V.abs()
+    want, bound = ((x.view(2, new, D).transpose(0, 1)) for x in (w @ V, bound))
+    for n_splits in (1, 2):
+        check(step.run(window, sinks, n_splits), want, bound, dtype, f"ctx {ctx} + {new} splits {n_splits}")
