@@ -3,9 +3,10 @@
 
 namespace kush {
 
-// One warp per (row, q head): o = sum_z exp(m_z - M) o_z / sum_z exp(m_z - M) l_z, lane z % 32 holding the factors of its
-// splits, the partial outputs read D/32 channels a lane.  Rows before the first sequence and behind the last one (before
-// qsl[0], from qsl[S] on; qsl null: none) have no partials and are left as they are.
+// One warp per (row, q head): o = sum_z e^(m_z - M) o_z / sum_z e^(m_z - M) l_z, lane z % 32 holding the factors of its splits,
+// the partial outputs read D/32 channels a lane.  The arithmetic is merge_splits' (sums in split order, fmaf, one division), so
+// that the windowed decode's output does not depend on which merge it takes.  Rows before the first sequence and behind the last
+// one (before qsl[0], from qsl[S] on; qsl null: none) have no partials and are left as they are.
 template <int D, class IN>
 __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out, const float* __restrict__ part_ml,
                                                             const float* __restrict__ part_o, int n_splits, int H, int G,
@@ -24,18 +25,22 @@ __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out
 #pragma unroll
     for (int i = 0; i < R; i++) o[i] = 0.0f;
     for (int z0 = 0; z0 < n_splits; z0 += WARP) {
-        float f = 0.0f;
+        float f = 0.0f, l = 0.0f;
+        bool part = false;                                                    // an empty split's partial output is not written
         if (z0 + lane < n_splits) {
             const float2 ml = *reinterpret_cast<const float2*>(part_ml + 2 * (first + int64_t(z0 + lane) * G));
-            if (ml.x > -INFINITY) {
-                f = exp2f((ml.x - M) * 1.4426950408889634f);
-                L += f * ml.y;
+            part = ml.x > -INFINITY;
+            if (part) {
+                f = __expf(ml.x - M);
+                l = ml.y;
             }
         }
+        const unsigned parts = __ballot_sync(0xffffffffu, part);
         const int nz = min(WARP, n_splits - z0);
         for (int z = 0; z < nz; z++) {
+            if (!(parts >> z & 1u)) continue;
             const float fz = __shfl_sync(0xffffffffu, f, z);
-            if (fz == 0.0f) continue;                                         // empty: its partial output is not written
+            L = fmaf(__shfl_sync(0xffffffffu, l, z), fz, L);
             const float* po = part_o + (first + int64_t(z0 + z) * G) * D + lane * R;
             float v[R];
             if constexpr (R == 2) {
@@ -48,10 +53,8 @@ __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out
             for (int i = 0; i < R; i++) o[i] = fmaf(fz, v[i], o[i]);
         }
     }
-    L = warp_sum(L);
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
-    for (int i = 0; i < R; i++) out[u * D + lane * R + i] = from_f32<IN>(o[i] * inv);
+    for (int i = 0; i < R; i++) out[u * D + lane * R + i] = from_f32<IN>(L > 0.0f ? o[i] / L : 0.0f);
 }
 
 int launch_chunk_combine(int D, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream) {

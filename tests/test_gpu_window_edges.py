@@ -59,3 +59,17 @@ def test_values_beside_a_sink(D, bits, G, dtype, P, gap, spread):
         print(f"gap {gap} spread {spread} splits {n_splits}: {worst:.3f} of the bound, rel {((got - want).norm() / want.norm()).item():.2e}, "
               f"bound {(bound.norm() / want.norm()).item():.2e}")
         assert worst <= 1.0, f"splits {n_splits}: {worst:.2f} times the bound"
+
+
+@pytest.mark.parametrize("D,bits,G,dtype,P,H,S", [(128, 4, 4, torch.bfloat16, 16, 2, 5), (128, 8, 7, torch.float16, 32, 1, 3),
+                                                  (64, 8, 1, torch.bfloat16, 16, 1, 1), (256, 4, 3, torch.float16, 32, 1, 1),
+                                                  (64, 4, 3, torch.float32, 16, 1, 3), (128, 4, 20, torch.bfloat16, 16, 1, 2)])
+@pytest.mark.parametrize("n_splits", [2, 3, 7, 33])
+@pytest.mark.parametrize("rotate", [False, True])
+def test_merges_agree(D, bits, G, dtype, P, H, S, n_splits, rotate):
+    """The merge in the decode launch and the one behind it give the same bits, wherever the partials lie in the work buffer."""
+    ops = ops_of(D, bits, G, dtype, P)
+    c = Cache(ops, [900, 33, 0, 411, 1200][:S], H, seed=3)
+    q = torch.randn(S, H * G, D, generator=torch.Generator().manual_seed(n_splits)).to(dtype).cuda()
+    got = [run(c, q, 700, 20, n_splits, fused, rotate=rotate) for fused in (False, True)]
+    assert not got[0].isnan().any() and torch.equal(*got)
