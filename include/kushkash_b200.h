@@ -200,6 +200,19 @@ int kush_sm100_attend_chunk(int32_t head_dim, int32_t bits, int32_t page, int32_
                             int32_t sinks, int32_t n_splits, float *part_ml, float *part_o, int64_t n_rows,
                             int32_t n_seqs, void *stream);
 
+/* kush_sm100_attend_chunk in which slot held_slot (0 or 1) of every block keeps back the weights of the held_tile-th key tile
+ * that it works on, and waits end after limit_ms (1 to 2000): blocks that reach that tile give up, raise bit 3 of
+ * kush_sm100_device_error and leave NaN in what they had not finished; the others give their outputs.  For tests of the bounded
+ * waits: head_dim 128, 4 bits, pages of 16, bf16. */
+int kush_sm100_attend_chunk_held(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group,
+                                 const void *q, int64_t q_stride, const void *k_new, const void *v_new, int64_t k_stride,
+                                 int64_t v_stride, void *out, const int32_t *query_start_loc, const int32_t *seq_lens,
+                                 const int32_t *tail_idx, const void *cache, int64_t block_stride, int64_t head_stride,
+                                 const void *tail_k, const int32_t *block_table, int64_t max_pages, int32_t hkv,
+                                 float scale, int32_t window, int32_t sinks, int32_t n_splits, float *part_ml,
+                                 float *part_o, int64_t n_rows, int32_t n_seqs, int32_t held_slot, int32_t held_tile,
+                                 int32_t limit_ms, void *stream);
+
 /* Rotary positions of `rows` rows of q (q_heads heads of head_dim) and k (k_heads; either count may be 0): channels
  * [0, rotary_dim) of a head turn in pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved, by positions[row]
  * (int32, or int64 if positions_64) times turns[i] / 2^64 of a full turn (device, rotary_dim / 2 entries; the product is
@@ -220,8 +233,8 @@ int kush_sm100_decode_tensor_cores(int32_t head_dim, int32_t bits, int32_t page,
 /* Bounded-wait watchdog of the kernels that wait: bit 0 set if a decode launch gave up waiting for a page copy (its
  * outputs were written as NaN), bit 1 if a bulk write gave up waiting for its input rows (the records of that
  * warp's remaining items were not written), bit 2 if a peer-gather wait gave up on a peer (kush_sm100_gather_wait:
- * the gathered outputs are incomplete), bit 3 if a chunk attention gave up a wait inside a block (that block's outputs
- * were written as NaN); 0 if none.  clear != 0 resets the flags.
+ * the gathered outputs are incomplete), bit 3 if a chunk attention gave up a wait inside a block (what that block had not
+ * finished was written as NaN); 0 if none.  clear != 0 resets the flags.
  * Synchronous (reads device variables); -1 on a CUDA error.  No counterpart in the reference, whose kernels have
  * no bounded waits. */
 int kush_sm100_device_error(int32_t clear);

@@ -51,6 +51,8 @@ SIGNATURES = {
                                  _i32, _p, _p, _p, _i32, _i32, _p, _i32, _i32, _p],
     "kush_sm100_attend_chunk": [_i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64,
                                 _p, _p, _i64, _i32, _f32, _i32, _i32, _i32, _p, _p, _i64, _i32, _p],
+    "kush_sm100_attend_chunk_held": [_i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64,
+                                     _p, _p, _i64, _i32, _f32, _i32, _i32, _i32, _p, _p, _i64, _i32, _i32, _i32, _i32, _p],
     "kush_sm100_rope": [_i32, _i32, _i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64, _i32,
                         _p, _i32, _p, _f32, _i64, _p],
     "kush_sm100_decode_tensor_cores": [_i32, _i32, _i32, _i32, _i32],
@@ -107,7 +109,7 @@ def check(rc: int, what: str) -> None:
 def device_error(clear: bool = True) -> int:
     """Bounded-wait flags since the last clear: bit 0 a decode launch gave up (its outputs are NaN), bit 1 a bulk
     write gave up (some of its records were not written), bit 2 a peer-gather wait gave up on a peer, bit 3 a
-    chunk attention gave up a wait (outputs of that block are NaN); 0 if none."""
+    chunk attention gave up a wait (what that block had not finished is NaN); 0 if none."""
     rc = lib().kush_sm100_device_error(int(clear))
     if rc < 0:
         raise RuntimeError("kush_sm100_device_error: CUDA error")

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(128) chunk_combine_kernel(IN* __restrict__ out
         }
     }
 #pragma unroll
-    for (int i = 0; i < R; i++) out[u * D + lane * R + i] = from_f32<IN>(L > 0.0f ? o[i] / L : 0.0f);
+    for (int i = 0; i < R; i++) out[u * D + lane * R + i] = from_f32<IN>(L > 0.0f ? o[i] / L : L);      // (0, or a NaN that came with a partial)
 }
 
 int launch_chunk_combine(int D, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream) {
@@ -75,14 +75,13 @@ int launch_chunk_combine(int D, int dtype, const AttendArgs& a, int64_t rows, cu
 
 using namespace kush;
 
-extern "C" int kush_sm100_attend_chunk(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group,
-                                       const void* q, int64_t q_stride, const void* k_new, const void* v_new,
-                                       int64_t k_stride, int64_t v_stride, void* out, const int32_t* query_start_loc,
-                                       const int32_t* seq_lens, const int32_t* tail_idx, const void* cache,
-                                       int64_t block_stride, int64_t head_stride, const void* tail_k,
-                                       const int32_t* block_table, int64_t max_pages, int32_t hkv, float scale,
-                                       int32_t window, int32_t sinks, int32_t n_splits, float* part_ml, float* part_o,
-                                       int64_t n_rows, int32_t n_seqs, void* stream) {
+static int attend_chunk(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group, const void* q, int64_t q_stride,
+                        const void* k_new, const void* v_new, int64_t k_stride, int64_t v_stride, void* out,
+                        const int32_t* query_start_loc, const int32_t* seq_lens, const int32_t* tail_idx, const void* cache,
+                        int64_t block_stride, int64_t head_stride, const void* tail_k, const int32_t* block_table,
+                        int64_t max_pages, int32_t hkv, float scale, int32_t window, int32_t sinks, int32_t n_splits,
+                        float* part_ml, float* part_o, int64_t n_rows, int32_t n_seqs, void* stream, int32_t held_slot = 0,
+                        int32_t held_tile = 0, int32_t limit_ms = 0) {
     static const char* what = "kush_sm100_attend_chunk";
     if (kush_sm100_record_bytes(head_dim, bits, page) == 0 || dtype < KUSH_F16 || dtype > KUSH_F32)
         return set_error(KUSH_ERR_UNSUPPORTED, "%s: unsupported head_dim %d / bits %d / page %d / dtype %d", what, head_dim,
@@ -133,9 +132,41 @@ extern "C" int kush_sm100_attend_chunk(int32_t head_dim, int32_t bits, int32_t p
     a.n_splits = n_splits;
     a.part_ml = part_ml;
     a.part_o = part_o;
+    a.held = {held_slot, held_tile, limit_ms};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int rc = attend_tc_supported(head_dim, dtype) ? launch_attend_tc(head_dim, bits, page, dtype, a, n_rows, st)
                                                         : launch_attend_simt(head_dim, bits, page, dtype, a, n_rows, st);
     if (rc != KUSH_OK || n_splits == 1) return rc;
     return launch_chunk_combine(head_dim, dtype, a, n_rows, st);
+}
+
+extern "C" int kush_sm100_attend_chunk(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group,
+                                       const void* q, int64_t q_stride, const void* k_new, const void* v_new,
+                                       int64_t k_stride, int64_t v_stride, void* out, const int32_t* query_start_loc,
+                                       const int32_t* seq_lens, const int32_t* tail_idx, const void* cache,
+                                       int64_t block_stride, int64_t head_stride, const void* tail_k,
+                                       const int32_t* block_table, int64_t max_pages, int32_t hkv, float scale,
+                                       int32_t window, int32_t sinks, int32_t n_splits, float* part_ml, float* part_o,
+                                       int64_t n_rows, int32_t n_seqs, void* stream) {
+    return attend_chunk(head_dim, bits, page, dtype, group, q, q_stride, k_new, v_new, k_stride, v_stride, out,
+                        query_start_loc, seq_lens, tail_idx, cache, block_stride, head_stride, tail_k, block_table, max_pages, hkv, scale, window, sinks,
+                        n_splits, part_ml, part_o, n_rows, n_seqs, stream);
+}
+
+extern "C" int kush_sm100_attend_chunk_held(int32_t head_dim, int32_t bits, int32_t page, int32_t dtype, int32_t group,
+                                            const void* q, int64_t q_stride, const void* k_new, const void* v_new,
+                                            int64_t k_stride, int64_t v_stride, void* out, const int32_t* query_start_loc,
+                                            const int32_t* seq_lens, const int32_t* tail_idx, const void* cache,
+                                            int64_t block_stride, int64_t head_stride, const void* tail_k,
+                                            const int32_t* block_table, int64_t max_pages, int32_t hkv, float scale,
+                                            int32_t window, int32_t sinks, int32_t n_splits, float* part_ml, float* part_o,
+                                            int64_t n_rows, int32_t n_seqs, int32_t held_slot, int32_t held_tile,
+                                            int32_t limit_ms, void* stream) {
+    if (held_slot < 0 || held_slot > 1 || held_tile < 0 || limit_ms < 1 || limit_ms > 2000)
+        return set_error(KUSH_ERR_ARG, "kush_sm100_attend_chunk_held: slot %d tile %d limit_ms %d", held_slot, held_tile, limit_ms);
+    if (head_dim != 128 || bits != 4 || page != 16 || dtype != KUSH_BF16)
+        return set_error(KUSH_ERR_UNSUPPORTED, "kush_sm100_attend_chunk_held: head_dim 128, 4 bits, pages of 16, bf16 only");
+    return attend_chunk(head_dim, bits, page, dtype, group, q, q_stride, k_new, v_new, k_stride, v_stride, out,
+                        query_start_loc, seq_lens, tail_idx, cache, block_stride, head_stride, tail_k, block_table, max_pages, hkv, scale, window, sinks,
+                        n_splits, part_ml, part_o, n_rows, n_seqs, stream, held_slot, held_tile, limit_ms);
 }

@@ -30,6 +30,8 @@ struct AttendArgs {
     int32_t n_splits;
     float *part_ml, *part_o;
     int32_t rot;                     // decode with rotation: q rotated as it loads, the output rotated back
+    // limit_ms > 0: this slot of every block keeps back its tile-th tile's weights, and waits end after limit_ms
+    struct { int32_t slot, tile, limit_ms; } held;
 };
 
 struct RowTile {

@@ -43,7 +43,8 @@
 //   20 warps, registers moved    ten producing warps of 88 registers by setmaxnreg: spills, 892 TFLOP/s; not kept
 // Short calls (20 rows a sequence) are bound by that chain: 64 sequences x 5 rows over 4000-8192 tokens 361 us.
 //
-// Waits are bounded (2 s): on a timeout the block raises the error flag, writes NaN and returns.
+// Waits are bounded (2 s): on a timeout the block raises the error flag, every warp leaves its loop, outputs that were not
+// complete by then become NaN (a partial's maximum +inf and sum NaN, which no merge drops), and the block returns.
 #include <atomic>
 
 #include "kush_async.cuh"
@@ -207,8 +208,8 @@ __device__ __forceinline__ bool mbar_done(uint32_t bar, uint32_t parity) {
     return ok;
 }
 // the rest of a wait: the warp sleeps in try_wait for up to 20 us at a time (polls would take issue slots from the
-// softmax); 2 s without the phase and the block gives up
-__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+// softmax); `limit` ns without the phase and the block gives up
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up, uint64_t limit) {
     uint64_t t0 = 0;
     for (;;) {
         uint32_t ok;
@@ -222,7 +223,7 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile i
         uint64_t now;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
         if (t0 == 0) t0 = now;
-        else if (now - t0 > 2000000000ull) {
+        else if (now - t0 > limit) {
             *gave_up = 1;
             atomicExch(&g_attend_error, 1);
             return false;
@@ -235,8 +236,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// grid (row tiles, Hkv, n_splits), block 512
-template <int D, int BITS, int P, class IN>
+// grid (row tiles, Hkv, n_splits), block 512.  HELD: one slot keeps back one tile's weights (a.held), so that waits run out.
+template <int D, int BITS, int P, class IN, bool HELD>
 __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) {
     using F = Fmt<D, BITS, P>;
     using U = Unit<D, BITS, P>;
@@ -285,7 +286,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     // bounded wait for the phase of `parity` of a barrier; false if this block gave up
-    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return mbar_done(bar, parity) || wait_long(bar, parity, gave_up); };
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        return mbar_done(bar, parity) || wait_long(bar, parity, gave_up, HELD ? a.held.limit_ms * 1000000ull : 2000000000ull);
+    };
     const int32_t* bt = a.block_table + int64_t(t.s) * a.max_pages;
     const uint8_t* hcache = a.cache + int64_t(h) * a.head_stride;
     const int full = t.ctx / P * P;                                                // cached tokens in finished pages
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             }
             fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(p_full + 8 * slot);
+            if (lane == 0 && !(HELD && slot == a.held.slot && n == a.held.tile)) bar_arrive(p_full + 8 * slot);
             n++;
         }
         // ---------------------------------------------------------------- the slot's output
@@ -507,7 +510,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             ok = __all_sync(0xffffffffu, wait(o_full + 8 * slot, 0));
             fence_after();
         }
-        // split: slot 1 hands its maximum, sum and output over (in the key buffers, no longer read)
+        // split: slot 1 hands its maximum, sum and output over (in the key buffers and, at 128 channels, the first value buffer's
+        // front; no longer read)
         float* xm = reinterpret_cast<float*>(sm + M::K);                           // [2][128] m, l
         float* xo = xm + 256;                                                      // [128][D + 4]
         if (!paired) {
@@ -530,6 +534,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             }
             asm volatile("bar.sync 1, %0;" ::"r"(2 * WARP * rows0) : "memory");
         }
+        // (another warp of the block gave up: o_full may have come without the last products, xo from slot 1 not at all)
+        ok = __all_sync(0xffffffffu, ok && *gave_up == 0);
         if (paired || slot == 0) {
             float mo = -INFINITY, f0 = 1.0f, f1 = 0.0f;
             if (!paired) {
@@ -578,8 +584,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             }
             if (real && a.n_splits > 1) {
                 // sum and output are in units of 2^(m - TC_UP); log2 units -> natural, for the combine
-                a.part_ml[2 * pr] = ok ? (m - TC_UP) * 0.69314718055994531f : 0.0f;
-                a.part_ml[2 * pr + 1] = l;
+                a.part_ml[2 * pr] = ok ? (m - TC_UP) * 0.69314718055994531f : INFINITY;
+                a.part_ml[2 * pr + 1] = ok ? l : NAN;
             }
         }
         fence_before();
@@ -760,7 +766,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             load(IC<1>{}, f, bl, vr);
         }
 #pragma unroll 1
-        for (int k = 0; k < mine && ok; k++) {
+        for (int k = 0; k < mine; k++) {
             const int x = w + n_prod * k, n = x >> 3, st = n & 1;
             const uint32_t dst = base + M::K + st * M::TILE + (x & 7) * 2048, before = ((n >> 1) - 1) & 1;
             int32_t f1 = 0, bl1 = 0;
@@ -773,16 +779,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
                 f1 = __shfl_sync(0xffffffffu, from, (k + 1) & 31);
                 bl1 = __shfl_sync(0xffffffffu, blk, (k + 1) & 31);
             }
-            ok = wait(k_empty + 8 * st, before);                                   // (a fresh barrier lets tiles 0 and 1 pass)
+            // (a fresh barrier lets tiles 0 and 1 pass; a buffer that is still read is not written when a wait runs out)
+            if (!__all_sync(0xffffffffu, wait(k_empty + 8 * st, before))) break;
             convert(IC<0>{}, f, kr, dst);
             fence_async();
             __syncwarp();
             if (lane == 0) bar_arrive(k_full + 8 * st);
             if (k + 1 < mine) load(IC<0>{}, f1, bl1, kr);
-            ok = ok && wait(v_empty + 8 * st, before);
+            if (!__all_sync(0xffffffffu, wait(v_empty + 8 * st, before))) break;
             convert(IC<1>{}, f, vr, dst + (M::V - M::K));
             fence_async();
-            ok = __all_sync(0xffffffffu, ok);
+            __syncwarp();
             if (lane == 0) bar_arrive(v_full + 8 * st);
             if (k + 1 < mine) load(IC<1>{}, f1, bl1, vr);
             f = f1;
@@ -873,28 +880,34 @@ int attend_error_flag(int clear) {
 
 int attend_tc_supported(int D, int dtype) { return (D == 64 || D == 128) && (dtype == KUSH_F16 || dtype == KUSH_BF16); }
 
+template <int D, int BITS, int P, class IN, bool HELD>
+static int launch_tc(const AttendArgs& a, int64_t tiles, cudaStream_t stream) {
+    auto kern = attend_tc_kernel<D, BITS, P, IN, HELD>;
+    constexpr int smem = TcSmem<D>::BYTES;
+    static std::atomic<unsigned long long> attr_set{0};                            // one bit per device: the attribute is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(attr_set.load() >> (dev & 63) & 1ull)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return set_error(KUSH_ERR_CUDA, "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+        attr_set |= 1ull << (dev & 63);
+    }
+    launch_pdl(kern, dim3(unsigned(tiles), a.H, a.n_splits), dim3(TC_THREADS), size_t(smem), stream, a);
+    return check_launch("attention (tensor cores)");
+}
+
 int launch_attend_tc(int D, int bits, int P, int dtype, const AttendArgs& a, int64_t rows, cudaStream_t stream) {
     const int64_t tiles = (rows * a.G + TC_TM - 1) / TC_TM + a.S;                  // at most one more per sequence
     if (tiles > 0x7fffffff || a.H > 65535 || a.n_splits > 65535)
         return set_error(KUSH_ERR_ARG, "attention: %lld row tiles, %d kv heads, %d splits", (long long)tiles, a.H, a.n_splits);
+    if (a.held.limit_ms > 0) {
+        if (D != 128 || bits != 4 || P != 16 || dtype != KUSH_BF16) return KUSH_ERR_UNSUPPORTED;
+        return launch_tc<128, 4, 16, __nv_bfloat16, true>(a, tiles, stream);
+    }
     return dispatch_fmt(D, bits, P, dtype, [&](auto Dc, auto Bc, auto Pc, auto in) -> int {
         using IN = decltype(in);
-        if constexpr (Dc.value == 256 || std::is_same_v<IN, float>) {
-            return KUSH_ERR_UNSUPPORTED;
-        } else {
-            auto kern = attend_tc_kernel<Dc.value, Bc.value, Pc.value, IN>;
-            constexpr int smem = TcSmem<Dc.value>::BYTES;
-            static std::atomic<unsigned long long> attr_set{0};                    // one bit per device: the attribute is per device
-            int dev = 0;
-            cudaGetDevice(&dev);
-            if (!(attr_set.load() >> (dev & 63) & 1ull)) {
-                const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-                if (e != cudaSuccess) return set_error(KUSH_ERR_CUDA, "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-                attr_set |= 1ull << (dev & 63);
-            }
-            launch_pdl(kern, dim3(unsigned(tiles), a.H, a.n_splits), dim3(TC_THREADS), size_t(smem), stream, a);
-            return check_launch("attention (tensor cores)");
-        }
+        if constexpr (Dc.value == 256 || std::is_same_v<IN, float>) return KUSH_ERR_UNSUPPORTED;
+        else return launch_tc<Dc.value, Bc.value, Pc.value, IN, false>(a, tiles, stream);
     });
 }
 
