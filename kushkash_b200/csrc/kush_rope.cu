@@ -5,7 +5,7 @@
 // Angles.  No cosine table is read: a frequency comes as turns per position in 64-bit fixed point, T_i = f_i / (2 pi)
 // * 2^64, so position * T_i modulo 2^64 (one wrapping integer multiply) is the angle's fraction of a turn, exact range
 // reduction included for every position; read as a signed number it lies in [-1/2, 1/2) turn and goes to sincospif
-// after one rounding to fp32.  A far position loses nothing (|error| <= |position| 2^-65 turns from T_i's rounding).
+// after one rounding to fp32.  A far position loses nothing (|error| <= |position| 2^-65 turns: T_i is the nearest integer).
 //
 // Bound: HBM (each row read once, written once).  A block computes the cosines and sines of its rows once, into
 // shared memory, and every thread keeps those of its pairs in registers while it walks the heads, two 16-byte vectors

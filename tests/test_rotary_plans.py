@@ -61,3 +61,36 @@ def test_yarn_factor(keys, factor):
 def test_refused_keys(scaling):
     with pytest.raises(ValueError, match="rotary"):
         rotary_frequencies(16, 10000.0, scaling)
+
+
+@pytest.mark.parametrize("r,theta,scaling", [(128, 500000.0, None), (64, 10000.0, None), (256, 1e6, {"rope_type": "linear", "factor": 3.0}),
+                                             (20, 150000.0, {"rope_type": "ntk", "factor": 5.0}), (2, 10000.0, None)])
+def test_turns_are_the_nearest_integers(r, theta, scaling):
+    """2^64 f / 2 pi in 80 digits, f = theta^(-2i/r): a plan's entry is within half a count (of one turn in 2^64)."""
+    import decimal
+
+    import torch
+
+    from kushkash_b200._rotary import make_rotary
+    plan = make_rotary(torch.device("cpu"), 256, r, theta, False, scaling)
+    with decimal.localcontext(decimal.Context(prec=80)):
+        pi = decimal.Decimal("3.1415926535897932384626433832795028841971693993751058209749445923078164062862089986")
+        factor = decimal.Decimal(scaling["factor"]) if scaling else 1
+        for i, bits in enumerate(plan.turns.tolist()):
+            log = -decimal.Decimal(2 * i) / r * decimal.Decimal(theta).ln()
+            if scaling and scaling["rope_type"] == "ntk":
+                log -= decimal.Decimal(2 * i) / (r - 2) * factor.ln()
+            elif scaling:
+                log -= factor.ln()
+            turns = log.exp() / (2 * pi) * 2 ** 64
+            assert abs(bits % 2 ** 64 - turns) <= decimal.Decimal("0.5000001")
+
+
+def test_refused_values():
+    for theta in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="rotary"):
+            rotary_frequencies(16, theta)
+    for scaling in ({"rope_type": "linear", "factor": math.inf}, {"rope_type": "linear", "factor": -2.0}, {**YARN, "beta_slow": -1},
+                    {**YARN, "original_max_position_embeddings": 0}):
+        with pytest.raises(ValueError, match="rotary"):
+            rotary_frequencies(16, 10000.0, scaling)
