@@ -22,6 +22,7 @@ or an unsupported configuration raises.
 """
 from __future__ import annotations
 
+import functools
 import os
 
 import torch
@@ -36,6 +37,7 @@ MIN_SPLIT_PAGES = 16
 LONG_SPLIT_PAGES = 100
 CHUNK_TILE = 256
 MIN_CHUNK_SPLIT = 256
+MIN_SIMT_SPLIT = 160
 _I32_MAX = 2 ** 31 - 1
 
 
@@ -285,12 +287,28 @@ class Ops:
         """Split-KV factor for this device (split_factor); under a window, of the pages a query sees."""
         if window is None:
             return split_factor(num_seqs, num_kv_heads, max_full_pages, self.sms)
+        tokens = min(max_full_pages * self.P, window + self.P + sinks)
+        if not self._tensor_cores:
+            # CUDA cores: a block per tile of 32 q heads, as many on an SM as its shared memory (30, 55 or 104 KB) admits; small
+            # splits pay, as a block is bound by its own tiles.  One sequence x 8 kv heads under 8192 tokens: 16 to 32 splits by
+            # the tensor cores' rule, 37 or 51 by this one: fp32 of 128 channels 128 -> 108 us, of 64
+            # 185 -> 89, 40 heads a kv head 224 -> 138; 4 x 8 of 4096 tokens 189 -> 140, 194 -> 101, 277 -> 250
+            units = max(1, num_seqs * num_kv_heads * -(-self.G // 32))
+            resident = {64: 7, 128: 4, 256: 2}[self.D]
+            return max(1, min(MAX_SPLITS, resident * self.sms // units, tokens // MIN_SIMT_SPLIT))
         # a windowed unit has few pages, so a second wave of CTAs costs as much as the first: count the CTAs that are resident
-        # at once with this configuration's registers (61 sequences x 4 kv heads of 34 int8 pages: one split 37 us, two 47)
-        wide = self.D == 256 or self.G > 8
-        resident = 4 if self.D == 64 and not wide else 2 if wide else 3 if self.bits == 8 and self.P == 32 else 4
-        pages = min(max_full_pages, -(-window // self.P) + 1 + -(-sinks // self.P))
-        return split_factor(num_seqs, num_kv_heads, pages, self.sms, resident)
+        # at once.  int8 pages of 32: 3 at head_dim 128 (61 sequences x 4 kv heads of 34 pages: one split 37 us, two 47), 1 at
+        # 256 (30 x 4 of 32 pages: one 39 us, two 50).  head_dim 64 with more than 8 heads has 4; counting two measured better
+        # (4 x 8 of 4096 tokens: 9 splits 25.8 us, 10 27.6; 61 x 4 of 1000: one 29.4, two 31.8)
+        large = self.bits == 8 and self.P == 32
+        resident = (1 if large else 2) if self.D == 256 else 2 if self.G > 8 else 3 if large and self.D == 128 else 4
+        return split_factor(num_seqs, num_kv_heads, min(max_full_pages, -(-window // self.P) + 1 + -(-sinks // self.P)), self.sms,
+                            resident)
+
+    @functools.cached_property
+    def _tensor_cores(self) -> bool:
+        """Whether the decode of this configuration runs on the tensor cores."""
+        return bool(_cuda.decode_tensor_cores(self.cfg))
 
     def work_size(self, num_seqs: int, num_kv_heads: int, n_splits: int, fused: bool = False) -> int:
         """fp32 elements of the split-KV work buffer: S * Hkv * n_splits * G * (D + 2), the (M, L) pairs first, then

@@ -75,3 +75,20 @@ def test_refused_work_of_a_fused_merge(ops):
     with pytest.raises(ValueError, match="decode"):                            # no room for the counters
         ops.decode(**arguments(n_splits=2, fused=True, work=torch.zeros(ops.work_size(S, H, 2))))
     assert not ops.calls
+
+
+@pytest.mark.parametrize("D,bits,G,dtype,page,seqs,heads,window,want", [
+    (128, 4, 4, torch.bfloat16, 16, 1, 8, 8192, 32), (128, 8, 7, torch.float16, 32, 61, 4, 1000, 1), (128, 8, 7, torch.float16, 32, 30, 4, 1000, 2),
+    (64, 4, 16, torch.bfloat16, 16, 4, 8, 4096, 9), (64, 4, 16, torch.bfloat16, 16, 61, 4, 1000, 1),      # two CTAs an SM, though four fit
+    (256, 8, 4, torch.bfloat16, 32, 4, 8, 4096, 4), (256, 8, 4, torch.bfloat16, 32, 30, 4, 1000, 1),      # one CTA an SM
+    (256, 4, 4, torch.bfloat16, 16, 4, 8, 4096, 9),
+    (128, 4, 4, torch.float32, 16, 4, 8, 4096, 18), (128, 4, 4, torch.float32, 16, 1, 8, 8192, 51),       # the CUDA cores' own rule
+    (128, 4, 40, torch.bfloat16, 32, 1, 8, 8192, 37), (64, 8, 4, torch.float32, 32, 61, 4, 1000, 4), (256, 4, 12, torch.bfloat16, 16, 61, 4, 1000, 1),
+    (256, 4, 1, torch.float32, 16, 1, 1, 100, 1), (64, 4, 1, torch.float32, 16, 0, 1, 100, 1)])
+def test_splits_follow_the_kernels(D, bits, G, dtype, page, seqs, heads, window, want):
+    from kushkash_b200 import GpuConfig, Ops
+    o = Ops.__new__(Ops)
+    o.D, o.bits, o.G, o.dtype, o.P, o.sms = D, bits, G, dtype, page, 148
+    o.cfg = GpuConfig(D, bits, G, str(dtype)[6:], "sm_100a", page)
+    assert o.splits(seqs, heads, 100000 // page, window=window) == want
+    assert o.splits(seqs, heads, 0, window=window) == 1
