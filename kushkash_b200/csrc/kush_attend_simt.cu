@@ -211,8 +211,11 @@ __global__ void __launch_bounds__(AS_THREADS) attend_simt_kernel(AttendArgs a) {
                 o[3] = acc[r][i].w;
             }
             if (tx == 0) {
-                a.part_ml[2 * pr] = mrow[row] * 0.69314718055994531f;        // log2 units -> natural, for the combine
-                a.part_ml[2 * pr + 1] = lrow[row];
+                // log2 units -> natural, for the combine; NaN scores leave the maximum as it was, +inf keeps the merge from dropping
+                // their part
+                const float l = lrow[row];
+                a.part_ml[2 * pr] = l == l ? mrow[row] * 0.69314718055994531f : INFINITY;
+                a.part_ml[2 * pr + 1] = l;
             }
         }
         return;

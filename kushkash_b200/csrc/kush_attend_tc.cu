@@ -584,8 +584,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
             }
             if (real && a.n_splits > 1) {
                 // sum and output are in units of 2^(m - TC_UP); log2 units -> natural, for the combine
-                a.part_ml[2 * pr] = ok ? (m - TC_UP) * 0.69314718055994531f : INFINITY;
-                a.part_ml[2 * pr + 1] = ok ? l : NAN;
+                const bool whole = ok && l == l;                                  // (NaN scores leave m as it was)
+                a.part_ml[2 * pr] = whole ? (m - TC_UP) * 0.69314718055994531f : INFINITY;
+                a.part_ml[2 * pr + 1] = whole ? l : NAN;
             }
         }
         fence_before();

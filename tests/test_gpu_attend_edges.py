@@ -122,3 +122,20 @@ def test_new_and_unfinished_keys_enter_as_they_are(dtype, D, bits, P, ctx, new, 
     want, bound = ((x.view(2, new, D).transpose(0, 1)) for x in (w @ V, bound))
     for n_splits in (1, 2):
         check(step.run(window, sinks, n_splits), want, bound, dtype, f"ctx {ctx} + {new} splits {n_splits}")
+
+
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16), (128, torch.float32), (256, torch.bfloat16)])
+def test_a_row_of_nan_stays_its_own(D, dtype):
+    """A query of NaN gives a row of NaN, split or not, and no other row changes."""
+    ops = ops_of(D, 4, 2, dtype, 16)
+    c = Cache(ops, [600], 2, seed=9)
+    step = Step(c, [40], seed=1, spare=0)
+    for n_splits in (1, 3):
+        want = step.run(None, 0, n_splits)
+        q = step.q.clone()
+        step.q[7, 1] = float("nan")
+        got = step.run(None, 0, n_splits)
+        step.q.copy_(q)
+        assert got[7, 1].isnan().all()
+        got[7, 1] = want[7, 1]
+        assert torch.equal(got, want)
