@@ -217,8 +217,8 @@ int kush_sm100_attend_chunk_held(int32_t head_dim, int32_t bits, int32_t page, i
  * [0, rotary_dim) of a head turn in pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved, by positions[row]
  * (int32, or int64 if positions_64) times turns[i] / 2^64 of a full turn (device, rotary_dim / 2 entries; the product is
  * taken modulo 2^64: exact for every position), times `factor`; the other channels are copied.  fp32 arithmetic, one
- * rounding.  Strides in elements; an output may be its input (same strides).  No counterpart kernel in the reference
- * (its callers rotate with torch before kush_append / kush_write). */
+ * rounding.  Strides in elements; an output may be its input (same strides), else it must not overlap one.  No counterpart
+ * kernel in the reference (its callers rotate with torch before kush_append / kush_write). */
 int kush_sm100_rope(int32_t head_dim, int32_t dtype, int32_t rotary_dim, int32_t interleaved, const void *q,
                     int64_t q_row_stride, int64_t q_head_stride, void *q_out, int64_t qo_row_stride,
                     int64_t qo_head_stride, int32_t q_heads, const void *k, int64_t k_row_stride,

@@ -251,7 +251,7 @@ class Ops:
         """Rotary positions of the rows of a step, before append() / write() / attend_chunk(): q [rows, Hq, D] and k
         [rows, H, D] (either may be None; row and head strides free, e.g. parts of q|k|v rows), row i at positions[i]
         (int32 or int64, contiguous), into q_out and k_out (new tensors, or q and k themselves, or others of their
-        shapes).  Returns (q_out, k_out).  Angles are exact to fp32 for every position; one rounding to the dtype."""
+        shapes that overlap neither).  Returns (q_out, k_out).  Angles are exact to fp32 for every position; one rounding to the dtype."""
         D, rows, dt = self.D, positions.shape[0] if positions.dim() == 1 else -1, self.dtype
         wide = positions.dtype == torch.int64
         if rows < 0 or not (wide or positions.dtype == torch.int32) or not positions.is_contiguous():
@@ -275,7 +275,12 @@ class Ops:
             if len(shape) != 3 or shape[0] != rows or shape[2] != D or shape != y.shape or xs[2] != 1 or ys[2] != 1:
                 raise ValueError(f"rope: rows must be [{rows}, heads, {D}] with contiguous channels, outputs of their inputs' "
                                  "shapes")
-            args += (x.data_ptr(), xs[0], xs[1], y.data_ptr(), ys[0], ys[1], shape[1])
+            px, py = x.data_ptr(), y.data_ptr()
+            if (rows > 1 and (ys[0] == 0 or (px == py and xs[0] != ys[0]))) or (
+                    shape[1] > 1 and (ys[1] == 0 or (px == py and xs[1] != ys[1]))):
+                raise ValueError("rope: an output must be its input with the same strides or lie apart from it, and have no "
+                                 "expanded dimension")
+            args += (px, xs[0], xs[1], py, ys[0], ys[1], shape[1])
             outs.append(y)
         self._run("kush_sm100_rope", D, self.cfg.dtype_code, rotary.rotary_dim, int(rotary.interleaved), *args,
                   positions.data_ptr(), int(wide), rotary.turns.data_ptr(), rotary.factor, rows)

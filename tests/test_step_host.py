@@ -1,0 +1,41 @@
+"""What rope and attend_chunk refuse before anything is launched, on CPU tensors: an Ops object whose launches are recorded."""
+import pytest
+import torch
+
+D, G, H, P, S, ROWS = 64, 2, 3, 16, 2, 5
+
+
+@pytest.fixture
+def ops():
+    from kushkash_b200 import GpuConfig, Ops
+    o = Ops.__new__(Ops)
+    o.device, o.dev = torch.device("cpu"), torch.zeros(1).get_device()
+    o.D, o.bits, o.G, o.dtype, o.P, o._fmt = D, 4, G, torch.float16, P, (D, 4, P, 0)
+    o.cfg = GpuConfig(D, 4, G, "float16", "sm_100a", P)
+    o.calls = []
+    o._run = lambda entry, *args: o.calls.append((entry, args))
+    return o
+
+
+def test_rope_outputs(ops):
+    plan, pos = ops.rotary(), torch.arange(ROWS)
+    x = torch.zeros(ROWS, H, D, dtype=torch.float16)
+    wide = torch.zeros(ROWS, 2 * H * D, dtype=torch.float16)
+    flat = torch.zeros(ROWS * H * D, dtype=torch.float16)
+    for q, q_out in ((x, None), (x, x), (x, torch.empty_like(x)), (wide[:, :H * D].view(ROWS, H, D), wide[:, H * D:].view(ROWS, H, D)),
+                     (wide[:, :H * D].view(ROWS, H, D), wide[:, :H * D].view(ROWS, H, D)),
+                     (x[:1].expand(ROWS, H, D), torch.empty_like(x))):
+        ops.rope(q, None, pos, plan, q_out)
+        assert ops.calls.pop()[0] == "kush_sm100_rope"
+    ops.rope(x[:1], None, pos[:1], plan, wide[:1, :H * D].view(1, H, D))
+    ops.rope(x[:1], None, pos[:1], plan, flat.view(ROWS, H, D)[:1])
+    ops.calls.clear()
+    for q, q_out in ((x, torch.zeros(1, H, D, dtype=torch.float16).expand(ROWS, H, D)),       # every row into one
+                     (x, torch.zeros(ROWS, 1, D, dtype=torch.float16).expand(ROWS, H, D)),
+                     (x[:1].expand(ROWS, H, D), x),                                           # the first row is read while it is written
+                     (flat.view(ROWS, H, D), flat.view(H, ROWS, D).transpose(0, 1))):         # the same memory in another order
+        with pytest.raises(ValueError, match="rope"):
+            ops.rope(q, None, pos, plan, q_out)
+        with pytest.raises(ValueError, match="rope"):
+            ops.rope(None, q, pos, plan, None, q_out)
+    assert not ops.calls
