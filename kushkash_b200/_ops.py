@@ -471,9 +471,12 @@ class Ops:
             raise ValueError("attend_chunk: out must be contiguous, of q's shape")
         if tuple(tail_k.shape[1:]) != (H, self.P, D) or not tail_k.is_contiguous():
             raise ValueError(f"attend_chunk: tail_k must be contiguous [slots, {H}, {self.P}, {D}]")
+        if cache.dim() < 2 or cache.shape[1] < H:
+            raise ValueError(f"attend_chunk: cache must hold the records of {H} kv heads, got {tuple(cache.shape)}")
         i32 = torch.int32
         if (not (query_start_loc.dtype == seq_lens.dtype == tail_idx.dtype == block_table.dtype == i32)
-                or tuple(query_start_loc.shape) != (S + 1,) or tail_idx.shape[0] < S or block_table.shape[0] < S
+                or tuple(query_start_loc.shape) != (S + 1,) or seq_lens.dim() != 1 or tail_idx.dim() != 1 or block_table.dim() != 2
+                or tail_idx.shape[0] < S or block_table.shape[0] < S
                 or not query_start_loc.is_contiguous() or not seq_lens.is_contiguous() or not tail_idx.is_contiguous()
                 or block_table.stride(1) != 1):
             raise ValueError("attend_chunk: query_start_loc [S + 1], seq_lens and tail_idx [S] must be contiguous int32, "

@@ -39,3 +39,26 @@ def test_rope_outputs(ops):
         with pytest.raises(ValueError, match="rope"):
             ops.rope(None, q, pos, plan, None, q_out)
     assert not ops.calls
+
+
+def arguments(**kw):
+    i32 = torch.int32
+    a = dict(q=torch.zeros(ROWS, H * G, D, dtype=torch.float16), k=torch.zeros(ROWS, H, D, dtype=torch.float16),
+             v=torch.zeros(ROWS, H, D, dtype=torch.float16), out=torch.zeros(ROWS, H * G, D, dtype=torch.float16),
+             query_start_loc=torch.tensor([0, 2, 5], dtype=i32), seq_lens=torch.ones(S, dtype=i32), tail_idx=torch.zeros(S, dtype=i32),
+             cache=torch.zeros(5, H, P * D + 4 * D + 4 * P, dtype=torch.uint8), block_table=torch.zeros(S, 2, dtype=i32),
+             tail_k=torch.zeros(S, H, P, D, dtype=torch.float16), scale=0.125)
+    a.update(kw)
+    return a
+
+
+def test_chunk_arguments(ops):
+    ops.attend_chunk(**arguments())
+    ops.attend_chunk(**arguments(cache=torch.zeros(5, H + 1, 1344, dtype=torch.uint8)))
+    assert len(ops.calls) == 2
+    for kw in (dict(cache=torch.zeros(5, H - 1, 1344, dtype=torch.uint8)), dict(cache=torch.zeros(5000, dtype=torch.uint8)),
+               dict(tail_idx=torch.zeros((), dtype=torch.int32)), dict(block_table=torch.zeros(2 * S, dtype=torch.int32)),
+               dict(seq_lens=torch.ones(S, 1, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="attend_chunk"):
+            ops.attend_chunk(**arguments(**kw))
+    assert len(ops.calls) == 2
