@@ -25,11 +25,13 @@
 // TAU = 4, 5, 6, 8 (steps 2^-35, 2^-34, 2^-33, 2^-31): ragged prefill 465, 462, 460, 455 us, windowed int8 338, 327, 325, 324.
 //
 // What bounds it.  A pair of 128-row tiles and a key tile are 32 products of 64 cycles (2048 cycles of tensor cores), 32768
-// exponentials at 16 a cycle (2048 cycles) and 32768 dequantized values, all on four schedulers: none of the three alone,
-// their sum of issue slots and the chain product -> softmax -> product do.  One wave of blocks (1152 rows of 4 q heads on 8
-// kv heads over 30001 int4 tokens, bf16) takes 616 us = 936 TFLOP/s, 57% of the measured bf16 GEMM rate; with the
-// conversions left out 556, the softmax's arithmetic left out 497, both 449.  8192 new rows without history: 628 us = 876.
-// What the design rests on, measured on that wave or on a 2048-row chunk:
+// exponentials at 16 a cycle (2048 cycles) and 32768 dequantized values.  No unit is full: over 6000 tokens the counters show
+// the tensor pipe 38% busy, the exponential pipe 38%, issue slots 44%, and waits for loads (long scoreboard, 3.9 per issued
+// instruction) as the largest stall: the latency of the chain product -> softmax -> product and of the producers' loads.  One
+// wave of blocks (1152 rows of 4 q heads on 8 kv heads over 30001 int4 tokens, bf16; 144 of 148 SMs) takes 622 us = 927
+// TFLOP/s, 56% of the measured bf16 GEMM rate; 8192 new rows without history 616 us = 892.  (When it took 616: with the
+// conversions left out 556, the softmax's arithmetic left out 497, both 449.)
+// What the design rests on, each step measured on that wave or on a 2048-row chunk as it was built:
 //   two slots                    one issuing warp per slot: with one for both, its waits and issue left the tensor cores idle
 //                                (4200 cycles a tile for itself); operands in uniform registers (elect.sync, shuffled
 //                                values): a product's issue fell from 80 to 20 cycles
@@ -38,10 +40,11 @@
 //   into registers               bulk copies in shared memory instead cost the producers more instructions than it saved
 //   one pass over S              32 columns at a time; masked scores are rewritten in TMEM first (rolled loops: the code of
 //                                all roles has to stay in the instruction caches; unrolled, 28% of the stalls were fetches)
-//   exponentials on the FMA pipe  4, 8, 12, 16 of 32 by a polynomial: 906, 886, 865, 840 TFLOP/s; not kept (issue, not the
-//                                exponential unit, is short)
+//   q ref off the scores         in a loop of its own for the one tile that mixes both kinds of keys; in the masking loop it
+//                                cost every row 20 to 30% (ragged prefill 557 us against 467)
+//   exponentials on the FMA pipe  4, 8, 12, 16 of 32 by a polynomial: 906, 886, 865, 840 TFLOP/s; not kept
 //   20 warps, registers moved    ten producing warps of 88 registers by setmaxnreg: spills, 892 TFLOP/s; not kept
-// Short calls (20 rows a sequence) are bound by that chain: 64 sequences x 5 rows over 4000-8192 tokens 361 us.
+// Short calls (20 rows a sequence) are bound by that chain: 64 sequences x 5 rows over 4000-8192 tokens 370 us.
 //
 // Waits are bounded (2 s): on a timeout the block raises the error flag, every warp leaves its loop, outputs that were not
 // complete by then become NaN (a partial's maximum +inf and sum NaN, which no merge drops), and the block returns.

@@ -192,7 +192,8 @@ extern "C" int kush_sm100_decode_window(int32_t head_dim, int32_t bits, int32_t 
                               stream, counters, window < KUSH_NO_POSITION ? window : KUSH_NO_POSITION,
                               sinks < KUSH_NO_POSITION ? sinks : KUSH_NO_POSITION);
     if (rc != KUSH_OK || n_splits == 1 || counters || n_seqs == 0) return rc;
-    // a warp per output row reads its splits' factors at once: one sequence, 16 splits: 16.7 -> 16.0 us with the decode
+    // a warp per output row reads its splits' factors at once (the same bits): one sequence, 16 splits, the step that brought it
+    // 16.7 -> 16.0 us with the decode
     if (!rot && aligned16(part_o) && (reinterpret_cast<uintptr_t>(part_ml) & 7) == 0) {
         AttendArgs a{};
         a.out = out;
