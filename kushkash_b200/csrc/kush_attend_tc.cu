@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(AttendArgs a) 
     const uint8_t* hcache = a.cache + int64_t(h) * a.head_stride;
     const int full = t.ctx / P * P;                                                // cached tokens in finished pages
     // the key reference: the bias of the first finished page that the row tile sees (the same for all its splits)
-    const int first = kt.a > 0 ? 0 : kt.lo / P * P;
+    const int first = kt.ns > 0 ? 0 : kt.lo / P * P;
     const bool have_ref = first < full;
     if (tid < D) {
         const uint8_t* rec = have_ref ? hcache + int64_t(bt[first / P]) * a.block_stride : nullptr;

@@ -80,7 +80,7 @@ def test_small_weights_beside_one_large_one(dtype, D, n, at, window, gap):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("D,bits,P,ctx,new,window,sinks", [(128, 4, 16, 70, 12, None, 0), (128, 8, 32, 300, 200, None, 0),
                                                            (64, 4, 16, 128, 140, None, 0), (64, 8, 32, 261, 30, 100, 3),
-                                                           (128, 8, 16, 5, 40, None, 0)])
+                                                           (128, 8, 16, 5, 40, None, 0), (128, 4, 16, 20, 5, 4, 3), (64, 8, 16, 40, 9, 3, 20)])
 def test_new_and_unfinished_keys_enter_as_they_are(dtype, D, bits, P, ctx, new, window, sinks):
     """Finished pages whose keys lie about 4000 in two channels, before new rows that do not: the new rows' keys must not lose
     what a shift by the pages' bias would round off.  q takes the two channels with opposite signs, so that the scores of the
