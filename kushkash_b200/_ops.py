@@ -38,6 +38,7 @@ LONG_SPLIT_PAGES = 100
 CHUNK_TILE = 256
 MIN_CHUNK_SPLIT = 256
 MIN_SIMT_SPLIT = 160
+MIN_SIMT_CHUNK_SPLIT = 48
 _I32_MAX = 2 ** 31 - 1
 
 
@@ -438,7 +439,18 @@ class Ops:
         (chunk_split_factor).  num_rows: the step's new rows; max_len: the longest sequence, new rows counted."""
         if window is not None:
             max_len = min(max_len, window + sinks + -(-num_rows // max(1, num_seqs)))
-        return chunk_split_factor(num_rows, num_seqs, num_kv_heads, self.G, max_len, self.sms)
+        if self.D != 256 and self.dtype != torch.float32:
+            return chunk_split_factor(num_rows, num_seqs, num_kv_heads, self.G, max_len, self.sms)
+        # CUDA cores: a block per 32 query rows, as many on an SM as its shared memory (30, 55 or 104 KB) admits.  Few blocks are
+        # split until they fill the SMs once, down to 48 tokens; many, whose waves are uneven, four times, in parts that pay for
+        # their merge.  By the tensor cores' rule and by this one, 8 kv heads of 4 q heads: a token over 8000 fp32 196 and 97 us,
+        # bf16 of 256 channels 282 and 157; 16 x 5 rows over 4000 fp32 of 128 channels 1559 and 558, of 64 1410 and 417, bf16 of 256
+        # 2274 and 1092; 300 rows over 4000 1196 and 1115, 857 and 681, 2723 and 2733
+        units = max(1, max(num_seqs, -(-num_rows * self.G // 32)) * num_kv_heads)
+        blocks = {64: 7, 128: 4, 256: 2}[self.D] * self.sms
+        if blocks // units >= 8:
+            return max(1, min(MAX_SPLITS, blocks // units, max_len // MIN_SIMT_CHUNK_SPLIT))
+        return max(1, min(MAX_SPLITS, 4 * blocks // units, max_len // MIN_CHUNK_SPLIT))
 
     def chunk_work_size(self, num_rows: int, num_kv_heads: int, n_splits: int) -> int:
         """fp32 elements of attend_chunk()'s work buffer for n_splits > 1: the unnormalised outputs of every row and

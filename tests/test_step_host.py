@@ -62,3 +62,17 @@ def test_chunk_arguments(ops):
         with pytest.raises(ValueError, match="attend_chunk"):
             ops.attend_chunk(**arguments(**kw))
     assert len(ops.calls) == 2
+
+
+@pytest.mark.parametrize("dim,dtype,seqs,rows,longest,window,want", [
+    (128, torch.bfloat16, 1, 17, 517, None, 2), (64, torch.float16, 16, 80, 4005, None, 1),        # tensor cores: chunk_split_factor
+    (128, torch.float32, 1, 17, 517, None, 10), (256, torch.bfloat16, 1, 17, 517, None, 10),       # 24 blocks of 32 rows
+    (128, torch.float32, 1, 1, 8001, None, 74), (256, torch.bfloat16, 1, 1, 8001, 1000, 20),       # filled once; the window's tokens
+    (64, torch.float32, 16, 80, 4005, None, 8), (128, torch.float32, 16, 80, 4005, None, 15),
+    (256, torch.float16, 16, 80, 4005, None, 9), (256, torch.bfloat16, 5, 500, 300, None, 1), (128, torch.float32, 1, 2048, 9000, None, 1),
+    (64, torch.float32, 0, 0, 0, None, 1)])
+def test_chunk_splits_follow_the_kernels(dim, dtype, seqs, rows, longest, window, want):
+    from kushkash_b200 import Ops
+    o = Ops.__new__(Ops)
+    o.D, o.G, o.dtype, o.sms = dim, 4, dtype, 148
+    assert o.chunk_splits(rows, seqs, 8, longest, window=window) == want
