@@ -139,3 +139,36 @@ def test_a_row_of_nan_stays_its_own(D, dtype):
         assert got[7, 1].isnan().all()
         got[7, 1] = want[7, 1]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.float16)])
+def test_two_streams_at_once(D, dtype):
+    """Chunk attention on two streams and the windowed decode beside them, with work buffers of their own: the same bits as one
+    after the other (blocks of two launches share an SM's tensor memory)."""
+    from kushkash_b200 import _cuda
+    ops = ops_of(D, 4, 4, dtype, 16)
+    c = Cache(ops, [900, 300, 1500], 4, seed=6)
+    steps = [Step(c, [200, 5, 60], seed=s, spare=0) for s in (1, 2)]
+    rows, dec = steps[0].q.shape[0], torch.randn(3, 16, D, device="cuda").to(dtype)
+    outs = [[torch.zeros(rows, 16, D, dtype=dtype, device="cuda") for _ in range(12)] for _ in steps]
+    works = [torch.zeros(ops.chunk_work_size(rows, 4, 3), device="cuda") for _ in steps]
+    outs.append([torch.zeros_like(dec) for _ in range(12)])
+
+    def call(i, out):
+        if i == 2:
+            ops.decode(dec, out, c.pool, c.block_table, c.seq_lens, c.tail_idx, c.tail_k, D ** -0.5, window=700, sinks=4)
+        else:
+            s = steps[i]
+            ops.attend_chunk(s.q, s.k, s.v, out, s.qsl, s.seq_lens, c.tail_idx, c.pool, c.block_table, c.tail_k, D ** -0.5, 3, works[i])
+
+    want = [torch.zeros_like(o[0]) for o in outs]
+    for i in range(3):
+        call(i, want[i])
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for n in range(12):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                call(i, outs[i][n])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(3) for o in outs[i]) and _cuda.device_error() == 0
